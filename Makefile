@@ -6,7 +6,9 @@ PKG := mdn-vae_amd
 SRC := $(wildcard $(PKG)/csrc/*.hip) $(wildcard $(PKG)/csrc/*.cpp)
 OBJ := $(patsubst $(PKG)/csrc/%,build/%.o,$(SRC))
 LIB := $(PKG)/lib/libmdnvae_hip.so
-CXXFLAGS := $(EXTRA) -O3 -std=c++17 -fPIC --offload-arch=$(ARCH) -Wall -Wno-unused-function -Iinclude
+# packed FP32 instructions off: some of their forms have returned wrong results on this hardware, without an error
+NOPKFP32 := -Xclang -target-feature -Xclang -packed-fp32-ops
+CXXFLAGS := $(EXTRA) -O3 -std=c++17 -fPIC --offload-arch=$(ARCH) $(NOPKFP32) -Wall -Wno-unused-function -Iinclude
 
 all: $(LIB)
 

@@ -702,6 +702,31 @@ int mdnvae_ssim(const float* a, const float* b, long count, int n, float data_ra
  * function/VAE_CNN_NN.py:341-379 (weighted_paths = 0: hop counts, as that script attaches no distance). */
 int mdnvae_graph_features(const float* mats, long count, int n, int weighted_paths, float* out, void* stream);
 
+/* ---- orthogonalised updates ----------------------------------------------------------------------
+ * The other optimizer for weight matrices (the reference trains with Adam, function/VAE_CNN_NN.py:204).
+ * Newton-Schulz iteration on each matrix G [rows][cols] of a batch, m = min(rows, cols):
+ *     X = G / max(|G|_F, eps) (transposed if rows > cols);  `steps` times: A = X X^T, X <- a X + (b A + c A^2) X
+ * out = X in G's shape and type.  x, out: [batch][rows][cols], fp32 or bf16 (`dtype`); out may be x.  A matrix that
+ * holds a NaN or an infinity gives NaN throughout; a zero matrix gives zeros.  terms = 3: fp32-level products
+ * (two fp16 parts per operand), 1: one product of the high parts (about 1e-3 of the result's norm: for 16-bit
+ * results).  Coefficients that could take a singular value in [0, 1] past 256 are refused.  Workspace: 256-byte
+ * aligned, sized by the query (0 where each matrix fits one workgroup). */
+enum { MDNVAE_F32 = 0, MDNVAE_BF16 = 1 };
+enum { MDNVAE_MUON_MAX_STEPS = 16 };
+size_t mdnvae_orthogonalize_workspace_bytes(long batch, long rows, long cols);
+int mdnvae_orthogonalize(const void* x, void* out, long batch, long rows, long cols, int dtype, int steps, float a, float b,
+                         float c, float eps, int terms, void* workspace, size_t workspace_bytes, void* stream);
+/* The optimizer step around it, for `count` matrices of any shapes (host arrays of device pointers and sizes):
+ *     M <- momentum M + g;  u = g + momentum M (nesterov) or M;  O = orthogonalize(u)
+ *     p <- (1 - lr weight_decay) p - lr s O,   s = 1 | sqrt(max(1, rows / cols)) | 0.2 sqrt(max(rows, cols))
+ * params and grads fp32 or bf16 (`dtype`), momenta fp32.  No two of the matrices may overlap.  Pointers need their
+ * element's alignment only. */
+enum { MDNVAE_MUON_SCALE_NONE = 0, MDNVAE_MUON_SCALE_SHAPE = 1, MDNVAE_MUON_SCALE_RMS = 2 };
+size_t mdnvae_muon_workspace_bytes(const long* rows, const long* cols, int count);
+int mdnvae_muon_step(void* const* params, const void* const* grads, float* const* momenta, const long* rows, const long* cols,
+                     int count, int dtype, float lr, float momentum, int nesterov, float weight_decay, int scale_mode, int steps,
+                     float a, float b, float c, float eps, int terms, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

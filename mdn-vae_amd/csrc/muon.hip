@@ -1,0 +1,1144 @@
+// Orthogonalised updates: the Newton-Schulz iteration on a gradient (or momentum) matrix and the optimizer step around
+// it.  The reference trains with Adam only (function/VAE_CNN_NN.py:204); this is the other optimizer for the same
+// matrices.
+//
+//     X_0 = G / max(|G|_F, eps)   (transposed if G is tall: m <= n below)
+//     A = X X^T,   B = b A + c A^2,   X <- a X + B X          `steps` times
+//
+// Numerics.  X is carried as two fp16 parts of X * 2^e (22 significand bits; the power of two comes from a bound on
+// the singular values, so no largest magnitude has to be found) and every product is h h + h l + l h on the fp16
+// matrix instruction, accumulated in fp32.  What the iteration amplifies (up to |a| = 3.4 times per step) is noise in
+// the directions of small singular values; B maps into the span of the large ones, so errors of A, of B and of the
+// product B X hardly reach those directions - only the rounding of X itself and of a X does.  The epilogue therefore
+// adds a X in fp32 from both parts.  Measured against float64 this is at or below the error of the same iteration in
+// plain fp32 (1e-6 .. 6e-6 of the norm, by spectrum).  For the same reason results of 16 bits need one product
+// of the high parts only (a X still from both): 0.3e-3 .. 1.9e-3 of the norm, next to 1.7e-3 of the result's own rounding.
+//
+// Layout.  A matrix [R][K] lives as tiles of 32 rows x 16 k, [R/32][K/16][part 2][32 rows x 32 bytes], the two
+// 16-byte halves of a row swapped where (row & 4): a 1 KiB tile is one LDS-DMA piece, a matrix operand with k along
+// the row is one ds_read_b128 per lane, and the operand with k down the column (X in B X) is two transposing
+// ds_read_b64_tr_b16 per lane of the same tile - so X needs no second, transposed copy.  Both read whole 128-byte
+// groups of banks.
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include "common.h"
+#include "../../include/mdnvae_hip.h"
+
+namespace mdnvae {
+
+typedef _Float16 mu_h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 mu_h4 __attribute__((ext_vector_type(4)));
+typedef short mu_s4 __attribute__((ext_vector_type(4)));
+typedef short mu_s8 __attribute__((ext_vector_type(8)));
+typedef float mu_acc __attribute__((ext_vector_type(16)));
+typedef float mu_f4 __attribute__((ext_vector_type(4)));
+
+constexpr int MU_FRAG = 1024;            // one part of one 32 x 16 tile
+constexpr int MU_STEP = 2 * MU_FRAG;     // both parts
+constexpr int MU_MAX = 32;               // table entries per launch (kernel arguments stay under 4 KB)
+constexpr int MU_NORM_BLOCK = 16384;     // entries of G per workgroup of the norm pass
+
+#define MU_GLOBAL_PTR(p) ((const __attribute__((address_space(1))) void*)(p))
+#define MU_LDS_PTR(p) ((__attribute__((address_space(3))) void*)(p))
+
+// One entry: `count` matrices of one shape.  Workspace of a matrix: X (two buffers, 4 mp np bytes each), A, B (4 mp mp
+// each), partial sums of A (splits > 1).  Matrix i of the entry starts at off + i * mu_matrix_bytes.
+struct MuGeo {
+    long off;
+    int m, n, mp, np;                    // m <= n, and padded to the tile
+    int trans;                           // the caller's matrix is [n][m]
+    int splits, kper;                    // of the k steps of X X^T
+    int count;
+};
+struct MuTab {
+    int n;
+    int start[MU_MAX + 1];               // first workgroup of each entry; INT_MAX past the last
+    MuGeo e[MU_MAX];
+};
+struct MuStarts { int s[MU_MAX + 1]; };
+// p: result or parameter, g: gradient (or the matrix itself), mom: momentum or null; matrix i at + i * stride elements
+struct MuPtrs {
+    void* p[MU_MAX];
+    const void* g[MU_MAX];
+    float* mom[MU_MAX];
+    float lr_scale[MU_MAX];
+};
+
+__host__ __device__ inline long mu_tri(int t) { return (long)t * (t + 1) / 2; }
+template <int TILE>
+__host__ __device__ inline long mu_partial_bytes(const MuGeo& g) {
+    return g.splits > 1 ? (long)g.splits * mu_tri(g.mp / TILE) * TILE * TILE * 4 : 0;
+}
+template <int TILE>
+__host__ __device__ inline long mu_matrix_bytes(const MuGeo& g) {
+    return 8L * g.mp * g.np + 8L * g.mp * g.mp + mu_partial_bytes<TILE>(g);
+}
+
+// entry of workgroup tl: all starts come in with a few wide scalar loads
+__device__ __forceinline__ int mu_entry(const MuTab& tab, int tl) {
+    int e = 0;
+#pragma unroll
+    for (int i = 1; i < MU_MAX; ++i) e += tl >= tab.start[i] ? 1 : 0;
+    return e;
+}
+
+template <typename T>
+__device__ __forceinline__ float mu_load(const T* p) { return (float)*p; }
+
+// u of one entry: with momentum, M <- mu M + g and u = g + mu M (Nesterov) or M; without, g itself
+struct MuMom { float mu; int nesterov; };
+template <typename T>
+__device__ __forceinline__ float mu_update(const T* g, float* mom, long i, const MuMom& mm, bool store) {
+    const float gv = (float)g[i];
+    if (!mom) return gv;
+    float m = mom[i];
+    if (store) {
+        m = mm.mu * m + gv;
+        mom[i] = m;
+    }
+    return mm.nesterov ? gv + mm.mu * m : m;
+}
+
+// ---- norm pass: momentum, and each workgroup's sum of squares (float64: the squares of finite fp32 numbers neither
+// overflow nor vanish) -------------------------------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(256) void mu_norm_kernel(MuTab tab, MuPtrs ptrs, MuMom mm, double* __restrict__ partial) {
+    __shared__ double red[4];
+    const int e = mu_entry(tab, blockIdx.x);
+    const MuGeo& ge = tab.e[e];
+    const long len = (long)ge.m * ge.n, per = (len + MU_NORM_BLOCK - 1) / MU_NORM_BLOCK;
+    const long local = blockIdx.x - tab.start[e], mat = local / per, blk = local - mat * per;
+    const T* g = static_cast<const T*>(ptrs.g[e]) + mat * len;
+    float* mom = ptrs.mom[e];
+    const long lo = blk * MU_NORM_BLOCK, hi = min(len, lo + MU_NORM_BLOCK);
+    double s = 0.0;
+#pragma unroll 8
+    for (long i = lo + threadIdx.x; i < hi; i += 256) {
+        const double u = (double)mu_update(g, mom, i, mm, true);
+        s += u * u;
+    }
+    s = block_sum<256, double>(s, red);
+    if (threadIdx.x == 0) partial[blockIdx.x] = s;
+}
+
+// 1 / max(|u|_F, eps) * scale; a norm that is not finite (an infinity or a NaN in the matrix) gives NaN, and with it a
+// result that is NaN throughout
+__device__ __forceinline__ double mu_inv_norm(double sum, float eps, float scale) {
+    if (!(sum <= 1.7e308)) return __longlong_as_double(0x7ff8000000000000LL);
+    return (double)scale / fmax(sqrt(sum), (double)eps);
+}
+
+__device__ __forceinline__ void mu_parts(float t, _Float16& h, _Float16& l) {
+    h = (_Float16)t;
+    l = (_Float16)(t - (float)h);
+}
+
+// byte offset of (row, 16-byte half) inside a tile
+__device__ __forceinline__ int mu_at(int row, int half) { return row * 32 + ((half ^ ((row >> 2) & 1)) << 4); }
+
+// ---- split pass: X_0 in parts; one workgroup = 32 rows x 64 columns of X, through LDS so that lanes run along the
+// caller's contiguous dimension ----------------------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(256) void mu_split_kernel(MuTab tab, MuStarts norm, MuPtrs ptrs, MuMom mm, float eps, float scale,
+                                                       const double* __restrict__ partial,
+                                                       char* __restrict__ ws, int tile128) {
+    __shared__ float tile[32][65];
+    __shared__ double red[4];
+    const int e = mu_entry(tab, blockIdx.x);
+    const MuGeo& ge = tab.e[e];
+    const int nt = ge.np / 64, per = (ge.mp / 32) * nt;
+    const int local = blockIdx.x - tab.start[e], mat = local / per, t = local - mat * per;
+    const int r0 = (t / nt) * 32, c0 = (t % nt) * 64;
+    const long len = (long)ge.m * ge.n, nper = (len + MU_NORM_BLOCK - 1) / MU_NORM_BLOCK;
+    const double* part = partial + norm.s[e] + mat * nper;
+    double s = 0.0;
+    for (long i = threadIdx.x; i < nper; i += 256) s += part[i];
+    s = wave_sum(s);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    const T* g = static_cast<const T*>(ptrs.g[e]) + mat * len;
+    float* mom = ptrs.mom[e];
+    if (!ge.trans) {
+        const int c = threadIdx.x & 63;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int r = (threadIdx.x >> 6) + 4 * k;
+            tile[r][c] = (r0 + r < ge.m && c0 + c < ge.n) ? mu_update(g, mom, (long)(r0 + r) * ge.n + c0 + c, mm, false) : 0.0f;
+        }
+    } else {
+        const int r = threadIdx.x & 31;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int c = (threadIdx.x >> 5) + 8 * k;
+            tile[r][c] = (r0 + r < ge.m && c0 + c < ge.n) ? mu_update(g, mom, (long)(c0 + c) * ge.m + r0 + r, mm, false) : 0.0f;
+        }
+    }
+    __syncthreads();
+    const double inv = mu_inv_norm((red[0] + red[1]) + (red[2] + red[3]), eps, scale);
+    const int r = threadIdx.x >> 3, c8 = threadIdx.x & 7;
+    mu_h8 hi, lo;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        _Float16 h, l;
+        mu_parts((float)((double)tile[r][c8 * 8 + k] * inv), h, l);
+        hi[k] = h;
+        lo[k] = l;
+    }
+    const long mb = tile128 ? mu_matrix_bytes<128>(ge) : mu_matrix_bytes<64>(ge);
+    char* dst = ws + ge.off + mat * mb + ((long)(r0 >> 5) * (ge.np >> 4) + (c0 >> 4) + (c8 >> 1)) * MU_STEP + mu_at(r, c8 & 1);
+    *reinterpret_cast<mu_h8*>(dst) = hi;
+    *reinterpret_cast<mu_h8*>(dst + MU_FRAG) = lo;
+}
+
+// ---- products --------------------------------------------------------------------------------------------------------
+// GRAM: A = X X^T (upper tiles, mirrored), POLY: B = b A + c A^2 (the same), STEP: X <- a X + B X.
+enum { MU_GRAM = 0, MU_POLY = 1, MU_STEP_X = 2 };
+
+struct MuScale {
+    float f_acc;       // what the accumulator is multiplied with (scales undone, the destination's applied, coefficient)
+    float f_add;       // what the tile already there (A in POLY, X in STEP) is multiplied with
+};
+
+__device__ __forceinline__ mu_h8 mu_tr(const char* p0, const char* p1) {
+    const mu_s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) mu_s4*)(p0));
+    const mu_s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) mu_s4*)(p1));
+    mu_s8 f;
+    f[0] = a[0]; f[1] = a[1]; f[2] = a[2]; f[3] = a[3];
+    f[4] = b[0]; f[5] = b[1]; f[6] = b[2]; f[7] = b[3];
+    return __builtin_bit_cast(mu_h8, f);
+}
+
+// lane offsets of the two ways to read an operand of 32 x 16 out of LDS
+struct MuLane {
+    int direct;        // rows of the tile are operand rows
+    int tr0, tr1;      // columns of two adjacent 16-row half tiles (512 bytes each) are operand rows
+};
+__device__ __forceinline__ MuLane mu_lane(int lane) {
+    MuLane o;
+    o.direct = mu_at(lane & 31, lane >> 5);
+    const int g = lane >> 4, n16 = g & 1, h = g >> 1, r = (lane & 15) >> 2, ch = lane & 3;
+    o.tr0 = n16 * 512 + (8 * h + r) * 32 + ((ch >> 1) << 4) + (ch & 1) * 8;
+    o.tr1 = n16 * 512 + (8 * h + 4 + r) * 32 + (((ch >> 1) ^ 1) << 4) + (ch & 1) * 8;
+    return o;
+}
+
+// acc += operand rows [TILE] x operand columns [TILE] over k steps [k0, k1).  Four waves (2 x 2), wave tile TILE/2 squared.
+// Ring of four stages, one k step each, filled by LDS-DMA three steps ahead; one counted wait and one barrier per step.
+// TR: the row operand is X read down its columns (rsrc: tile (0, first n step), nsteps: n steps of a row of tiles).
+template <int TILE, int TERMS, bool TR>
+__device__ __forceinline__ void mu_mainloop(const char* rsrc, const char* csrc, int nsteps, int KS, int k0, int k1, char* smem,
+                                            mu_acc (&acc)[TILE / 64][TILE / 64]) {
+    constexpr int F = TILE / 32, W = TILE / 64;          // tiles per side, of the workgroup and of a wave
+    constexpr int NP = TERMS == 3 ? 2 : 1;
+    constexpr int SIDE = F * NP, PPW = 2 * SIDE / 4;     // pieces of one side, pieces per wave
+    constexpr int STAGE = 2 * SIDE * MU_FRAG, NBUF = 4;
+    const int lane = threadIdx.x & 63;
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wr = wid >> 1, wc = wid & 1;
+    const MuLane ln = mu_lane(lane);
+    const char* src[PPW];
+    bool tr[PPW];
+#pragma unroll
+    for (int i = 0; i < PPW; ++i) {
+        const int q = wid + 4 * i, side = q / SIDE, f = (q % SIDE) / NP, part = (q % SIDE) % NP;
+        tr[i] = TR && side == 0;
+        if (tr[i]) src[i] = rsrc + (2L * f + (lane >> 5)) * MU_STEP + part * MU_FRAG + (lane & 31) * 16;
+        else src[i] = (side == 0 ? rsrc : csrc) + (long)f * KS * MU_STEP + part * MU_FRAG + lane * 16;
+    }
+    auto stage = [&](int buf, int ks) {
+#pragma unroll
+        for (int i = 0; i < PPW; ++i) {
+            const long at = tr[i] ? (long)(ks >> 1) * nsteps * MU_STEP + (ks & 1) * 512 : (long)ks * MU_STEP;
+            __builtin_amdgcn_global_load_lds(MU_GLOBAL_PTR(src[i] + at), MU_LDS_PTR(smem + buf * STAGE + (wid + 4 * i) * MU_FRAG),
+                                             16, 0, 0);
+        }
+    };
+    auto compute = [&](int buf) {
+        const char* sr = smem + buf * STAGE + wr * W * NP * MU_FRAG;
+        const char* sc = smem + buf * STAGE + (SIDE + wc * W * NP) * MU_FRAG;
+        mu_h8 r[W][NP], c[W][NP];
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+#pragma unroll
+            for (int s = 0; s < NP; ++s) {
+                c[i][s] = *reinterpret_cast<const mu_h8*>(sc + (i * NP + s) * MU_FRAG + ln.direct);
+                const char* t = sr + (i * NP + s) * MU_FRAG;
+                if constexpr (TR) r[i][s] = mu_tr(t + ln.tr0, t + ln.tr1);
+                else r[i][s] = *reinterpret_cast<const mu_h8*>(t + ln.direct);
+            }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                if constexpr (TERMS == 3) {              // smallest terms first
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[i][1], c[j][0], acc[i][j], 0, 0, 0);
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[i][0], c[j][1], acc[i][j], 0, 0, 0);
+                }
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[i][0], c[j][0], acc[i][j], 0, 0, 0);
+            }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const int nk = k1 - k0;
+    if (nk <= 0) return;
+    // past the end the last step is fetched again, into a buffer nobody reads any more: every wave always has the same
+    // number of operations in flight, and one counted wait fits every iteration
+#pragma unroll
+    for (int s = 0; s < NBUF - 1; ++s) stage(s, k0 + min(s, nk - 1));
+    for (int it = 0; it < nk; ++it) {
+        // own pieces of step `it` have landed, own reads of step it - 1 are done; after the barrier everybody's
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NBUF - 2) * PPW) : "memory");
+        stage((it + NBUF - 1) % NBUF, k0 + min(it + NBUF - 1, nk - 1));
+        compute(it % NBUF);
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the epilogue reuses the stages
+}
+
+// accumulator register e of a 32 x 32 block: row (e & 3) + 8 (e >> 2) + 4 (lane >> 5), column lane & 31.
+// Block with its first row at k = kr (of the destination's row) and columns = rows of destination row tile `rt`:
+// four consecutive k per register group leave as 8 bytes per part.
+__device__ __forceinline__ long mu_block_at(int rt, int KS, int kr, int q, int lane) {
+    const int col = lane & 31, h = lane >> 5;
+    return ((long)rt * KS + (kr >> 4) + (q >> 1)) * MU_STEP + mu_at(col, q & 1) + h * 8;
+}
+template <int NP>
+__device__ __forceinline__ void mu_put(char* at, const float (&v)[4]) {
+    mu_h4 hi, lo;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        _Float16 h, l;
+        mu_parts(v[k], h, l);
+        hi[k] = h;
+        lo[k] = l;
+    }
+    *reinterpret_cast<mu_h4*>(at) = hi;
+    if constexpr (NP == 2) *reinterpret_cast<mu_h4*>(at + MU_FRAG) = lo;
+}
+template <int NP>
+__device__ __forceinline__ void mu_get(const char* at, float (&v)[4]) {
+    const mu_h4 hi = *reinterpret_cast<const mu_h4*>(at);
+    mu_h4 lo = {0, 0, 0, 0};
+    if constexpr (NP == 2) lo = *reinterpret_cast<const mu_h4*>(at + MU_FRAG);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = (float)hi[k] + (float)lo[k];
+}
+
+// LDS written by some lanes of the wave, read by others: the hardware keeps a wave's LDS operations in order, the
+// compiler has to be told
+__device__ __forceinline__ void mu_wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// a tile of a symmetric matrix (tile row ti of k, tile column tj of rows), and its mirror image: transposed per 32 x 32
+// block through 4 KiB of LDS that belong to the wave
+template <int TILE, int TERMS, bool POLY>
+__device__ __forceinline__ void mu_emit_sym(mu_acc (&acc)[TILE / 64][TILE / 64], char* dst, const char* add, int KS, int ti, int tj,
+                                            const MuScale& sc, char* smem) {
+    constexpr int W = TILE / 64, NP = TERMS == 3 ? 2 : 1, F = TILE / 32;
+    const int lane = threadIdx.x & 63;
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wr = wid >> 1, wc = wid & 1, col = lane & 31, h = lane >> 5;
+    char* mine = smem + wid * 4096;
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            const int rb = ti * F + wr * W + i, cb = tj * F + wc * W + j;       // 32-blocks: k of the direct image, rows
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float v[4], old[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const long at = mu_block_at(cb, KS, rb * 32, q, lane);
+                if constexpr (POLY) mu_get<NP>(add + at, old);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = acc[i][j][4 * q + k] * sc.f_acc + (POLY ? old[k] * sc.f_add : 0.0f);
+                mu_put<NP>(dst + at, v);
+                if (ti != tj) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int row = 8 * q + 4 * h + k;
+                        _Float16 hi, lo;
+                        mu_parts(v[k], hi, lo);
+                        char* t = mine + (col >> 4) * 1024 + mu_at(row, (col >> 3) & 1) + (col & 7) * 2;
+                        *reinterpret_cast<_Float16*>(t) = hi;
+                        if constexpr (NP == 2) *reinterpret_cast<_Float16*>(t + 2048) = lo;
+                    }
+                }
+            }
+            if (ti != tj) {
+                mu_wave_fence();
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int p = 0; p < NP; ++p) {
+                        const mu_h8 v = *reinterpret_cast<const mu_h8*>(mine + p * 2048 + s * 1024 + lane * 16);
+                        *reinterpret_cast<mu_h8*>(dst + ((long)rb * KS + cb * 2 + s) * MU_STEP + p * MU_FRAG + lane * 16) = v;
+                    }
+                mu_wave_fence();
+            }
+        }
+}
+
+// tile t of the upper triangle, column by column: (i <= j)
+__device__ __forceinline__ void mu_pair(int t, int& i, int& j) {
+    j = (int)((sqrtf(8.0f * (float)t + 1.0f) - 1.0f) * 0.5f);
+    while ((j + 1) * (j + 2) / 2 <= t) ++j;
+    while (j * (j + 1) / 2 > t) --j;
+    i = t - j * (j + 1) / 2;
+}
+
+// workgroups of one XCD (every eighth) take consecutive tiles, which share operand panels through its L2
+__device__ __forceinline__ int mu_tile_index(int total) {
+    const int chunk = (total + 7) >> 3;
+    const int t = (blockIdx.x & 7) * chunk + (blockIdx.x >> 3);
+    return t < total ? t : -1;
+}
+
+template <int TILE, int TERMS, int MODE>
+__global__ __launch_bounds__(256) void mu_sym_kernel(MuTab tab, int total, char* __restrict__ ws, int ping, MuScale sc) {
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    const int tl = mu_tile_index(total);
+    if (tl < 0) return;
+    const int e = mu_entry(tab, tl);
+    const MuGeo& ge = tab.e[e];
+    const int T = ge.mp / TILE, ntri = T * (T + 1) / 2;
+    const int splits = MODE == MU_GRAM ? ge.splits : 1;
+    const int local = tl - tab.start[e], mat = local / (ntri * splits), rest = local - mat * ntri * splits;
+    const int s = rest / ntri, t = rest - s * ntri;
+    int ti, tj;
+    mu_pair(t, ti, tj);
+    char* base = ws + ge.off + mat * mu_matrix_bytes<TILE>(ge);
+    const long xs = 4L * ge.mp * ge.np, as = 4L * ge.mp * ge.mp;
+    char* A = base + 2 * xs;
+    const int KS = MODE == MU_GRAM ? ge.np >> 4 : ge.mp >> 4;
+    const char* src = MODE == MU_GRAM ? base + ping * xs : A;
+    const int k0 = s * ge.kper, k1 = MODE == MU_GRAM ? min(KS, k0 + ge.kper) : KS;
+    mu_acc acc[TILE / 64][TILE / 64];
+#pragma unroll
+    for (int i = 0; i < TILE / 64; ++i)
+#pragma unroll
+        for (int j = 0; j < TILE / 64; ++j)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) acc[i][j][k] = 0.0f;
+    const long rows = (long)(TILE / 32) * KS * MU_STEP;
+    mu_mainloop<TILE, TERMS, false>(src + ti * rows, src + tj * rows, 0, KS, MODE == MU_GRAM ? k0 : 0, k1, smem, acc);
+    if (MODE == MU_GRAM && splits > 1) {
+        // this split's share, as the registers lie (the reducing kernel has the same lanes): 256 bytes per store
+        float* part = reinterpret_cast<float*>(A + 2 * as) + ((long)s * ntri + t) * TILE * TILE;
+        const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+#pragma unroll
+        for (int i = 0; i < TILE / 64; ++i)
+#pragma unroll
+            for (int j = 0; j < TILE / 64; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    mu_f4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                    reinterpret_cast<mu_f4*>(part)[((wid * (TILE / 64) + i) * (TILE / 64) + j) * 256 + q * 64 + lane] = v;
+                }
+        return;
+    }
+    mu_emit_sym<TILE, TERMS, MODE == MU_POLY>(acc, MODE == MU_POLY ? A + as : A, A, ge.mp >> 4, ti, tj, sc, smem);
+}
+
+// the sum of the splits in fixed order, then what the product kernel does when there is one
+template <int TILE, int TERMS>
+__global__ __launch_bounds__(256) void mu_reduce_kernel(MuTab tab, char* __restrict__ ws, MuScale sc) {
+    __shared__ __attribute__((aligned(1024))) char smem[4 * 4096];
+    const int e = mu_entry(tab, blockIdx.x);
+    const MuGeo& ge = tab.e[e];
+    if (ge.splits == 1) return;
+    const int T = ge.mp / TILE, ntri = T * (T + 1) / 2;
+    const int local = blockIdx.x - tab.start[e], mat = local / ntri, t = local - mat * ntri;
+    int ti, tj;
+    mu_pair(t, ti, tj);
+    char* base = ws + ge.off + mat * mu_matrix_bytes<TILE>(ge);
+    const long xs = 4L * ge.mp * ge.np, as = 4L * ge.mp * ge.mp;
+    char* A = base + 2 * xs;
+    const float* part = reinterpret_cast<const float*>(A + 2 * as) + (long)t * TILE * TILE;
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    mu_acc acc[TILE / 64][TILE / 64];
+#pragma unroll
+    for (int i = 0; i < TILE / 64; ++i)
+#pragma unroll
+        for (int j = 0; j < TILE / 64; ++j)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) acc[i][j][k] = 0.0f;
+    for (int s = 0; s < ge.splits; ++s) {
+        const mu_f4* p = reinterpret_cast<const mu_f4*>(part + (long)s * ntri * TILE * TILE);
+#pragma unroll
+        for (int i = 0; i < TILE / 64; ++i)
+#pragma unroll
+            for (int j = 0; j < TILE / 64; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const mu_f4 v = p[((wid * (TILE / 64) + i) * (TILE / 64) + j) * 256 + q * 64 + lane];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) acc[i][j][4 * q + k] += v[k];
+                }
+    }
+    mu_emit_sym<TILE, TERMS, false>(acc, A, nullptr, ge.mp >> 4, ti, tj, sc, smem);
+}
+
+// where a finished result goes: out = v, or the parameter step p <- decay p - lr_scale v (one rounding to T)
+template <typename T>
+__device__ __forceinline__ void mu_finish(T* p, long i, float v, float decay, float lr_scale, bool step) {
+    p[i] = (T)(step ? decay * (float)p[i] - lr_scale * v : v);
+}
+
+// STEP: D rows = 128 (64) columns n of X, D columns = rows m, so that a lane's four consecutive rows are consecutive in X's
+// tiles.  LAST: the result leaves in the caller's layout and type.
+template <typename T, int TILE, int TERMS, bool LAST>
+__global__ __launch_bounds__(256) void mu_step_kernel(MuTab tab, int total, MuPtrs ptrs, char* __restrict__ ws, int ping, MuScale sc,
+                                                      float decay, int is_step) {
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    const int tl = mu_tile_index(total);
+    if (tl < 0) return;
+    const int e = mu_entry(tab, tl);
+    const MuGeo& ge = tab.e[e];
+    const int TM = ge.mp / TILE, TN = ge.np / TILE;
+    const int local = tl - tab.start[e], mat = local / (TM * TN), rest = local - mat * TM * TN;
+    const int tn = rest / TM, tm = rest - tn * TM;
+    char* base = ws + ge.off + mat * mu_matrix_bytes<TILE>(ge);
+    const long xs = 4L * ge.mp * ge.np, as = 4L * ge.mp * ge.mp;
+    const char* X = base + ping * xs;
+    char* Y = base + (ping ^ 1) * xs;
+    const char* B = base + 2 * xs + as;
+    const int NS = ge.np >> 4, KS = ge.mp >> 4;
+    constexpr int W = TILE / 64, F = TILE / 32;
+    mu_acc acc[W][W];
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) acc[i][j][k] = 0.0f;
+    mu_mainloop<TILE, TERMS, true>(X + (long)tn * (TILE / 16) * MU_STEP, B + (long)tm * F * KS * MU_STEP, NS, KS, 0, KS, smem, acc);
+    const int lane = threadIdx.x & 63;
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wr = wid >> 1, wc = wid & 1, h = lane >> 5;
+    const long len = (long)ge.m * ge.n;
+    T* out = LAST ? static_cast<T*>(ptrs.p[e]) + mat * len : nullptr;
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            const int nb = tn * F + wr * W + i, mb = tm * F + wc * W + j;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const long at = mu_block_at(mb, NS, nb * 32, q, lane);
+                float v[4], x[4];
+                mu_get<2>(X + at, x);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = acc[i][j][4 * q + k] * sc.f_acc + x[k] * sc.f_add;
+                if constexpr (!LAST) {
+                    mu_put<2>(Y + at, v);
+                } else {
+                    const int m = mb * 32 + (lane & 31), n = nb * 32 + 8 * q + 4 * h;
+                    if (m < ge.m) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (n + k < ge.n)
+                                mu_finish(out, ge.trans ? (long)(n + k) * ge.m + m : (long)m * ge.n + n + k, v[k], decay,
+                                          ptrs.lr_scale[e], is_step != 0);
+                    }
+                }
+            }
+        }
+}
+
+// ---- small matrices: the whole step in one workgroup ----------------------------------------------------------------------
+// X and A in parts fit LDS (mp np + mp mp <= 38912 entries, mp and np multiples of 32): norm, all iterations and the
+// parameter step in one launch, one matrix per workgroup of 16 waves.  A 32 x 32 block of a product belongs to one
+// wave; its registers are held until a barrier says that everybody has read what they overwrite.
+constexpr int MU_SMALL_ENTRIES = 38912;
+constexpr int MU_SMALL_NT = 1024;
+constexpr int MU_SMALL_BLOCKS = (MU_SMALL_ENTRIES / 1024 + 15) / 16;      // 32 x 32 blocks of X per wave
+constexpr int MU_SMALL_CHUNKS = (MU_SMALL_ENTRIES / 8 + MU_SMALL_NT - 1) / MU_SMALL_NT;
+
+struct MuSteps {                                   // per iteration: the three products' scales
+    int steps;
+    MuScale gram[MDNVAE_MUON_MAX_STEPS], poly[MDNVAE_MUON_MAX_STEPS], step[MDNVAE_MUON_MAX_STEPS];
+};
+
+template <typename T, int TERMS>
+__global__ __launch_bounds__(MU_SMALL_NT) void mu_small_kernel(MuTab tab, MuPtrs ptrs, MuMom mm, float eps, float x_scale, MuSteps st,
+                                                               float decay, int is_step) {
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    __shared__ double red[MU_SMALL_NT / 64];
+    constexpr int NP = TERMS == 3 ? 2 : 1;
+    const int e = mu_entry(tab, blockIdx.x);
+    const MuGeo& ge = tab.e[e];
+    const long len = (long)ge.m * ge.n;
+    const long mat = blockIdx.x - tab.start[e];
+    const T* g = static_cast<const T*>(ptrs.g[e]) + mat * len;
+    float* mom = ptrs.mom[e];
+    T* out = static_cast<T*>(ptrs.p[e]) + mat * len;
+    const int NS = ge.np >> 4, KS = ge.mp >> 4, MB = ge.mp >> 5, NB = ge.np >> 5;
+    char* X = smem;
+    char* A = smem + 4 * ge.mp * ge.np;
+    const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
+    const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const MuLane ln = mu_lane(lane);
+
+    {   // G (momentum) in, eight columns of a row per chunk
+        float u[MU_SMALL_CHUNKS][8];
+        const int per_row = ge.np >> 3, chunks = ge.mp * per_row;
+        double s = 0.0;
+#pragma unroll
+        for (int c = 0; c < MU_SMALL_CHUNKS; ++c) {
+            const int ch = tid + c * MU_SMALL_NT;
+            const int r = ch / per_row, c0 = (ch - r * per_row) * 8;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                u[c][k] = 0.0f;
+                if (ch < chunks && r < ge.m && c0 + k < ge.n) {
+                    u[c][k] = mu_update(g, mom, ge.trans ? (long)(c0 + k) * ge.m + r : (long)r * ge.n + c0 + k, mm, true);
+                    s += (double)u[c][k] * (double)u[c][k];
+                }
+            }
+        }
+        s = wave_sum(s);
+        if (lane == 0) red[wid] = s;
+        __syncthreads();
+        s = 0.0;
+#pragma unroll
+        for (int i = 0; i < MU_SMALL_NT / 64; ++i) s += red[i];
+        const double inv = mu_inv_norm(s, eps, x_scale);
+#pragma unroll
+        for (int c = 0; c < MU_SMALL_CHUNKS; ++c) {
+            const int ch = tid + c * MU_SMALL_NT;
+            if (ch < chunks) {
+                const int r = ch / per_row, c8 = ch - r * per_row;
+                mu_h8 hi, lo;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    _Float16 a, b;
+                    mu_parts((float)((double)u[c][k] * inv), a, b);
+                    hi[k] = a;
+                    lo[k] = b;
+                }
+                char* dst = X + ((r >> 5) * NS + (c8 >> 1)) * MU_STEP + mu_at(r & 31, c8 & 1);
+                *reinterpret_cast<mu_h8*>(dst) = hi;
+                *reinterpret_cast<mu_h8*>(dst + MU_FRAG) = lo;
+            }
+        }
+        __syncthreads();
+    }
+
+    // one 32 x 32 block: rows of `rows` (tile rb) times rows of `cols` (tile cb), or the columns of X (TR)
+    auto mfma = [&](const mu_h8 (&r)[NP], const mu_h8 (&c)[NP], mu_acc& acc) {
+        if constexpr (TERMS == 3) {
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[1], c[0], acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[0], c[1], acc, 0, 0, 0);
+        }
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[0], c[0], acc, 0, 0, 0);
+    };
+    auto zero = [](mu_acc& acc) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) acc[k] = 0.0f;
+    };
+    auto product = [&](const char* rows, const char* cols, int K, mu_acc& acc) {
+        zero(acc);
+        for (int ks = 0; ks < K; ++ks) {
+            mu_h8 r[NP], c[NP];
+#pragma unroll
+            for (int s = 0; s < NP; ++s) {
+                r[s] = *reinterpret_cast<const mu_h8*>(rows + ks * MU_STEP + s * MU_FRAG + ln.direct);
+                c[s] = *reinterpret_cast<const mu_h8*>(cols + ks * MU_STEP + s * MU_FRAG + ln.direct);
+            }
+            mfma(r, c, acc);
+        }
+    };
+    for (int it = 0; it < st.steps; ++it) {
+        // A = X X^T (at most 16 blocks: one per wave)
+        mu_acc acc;
+        const int rb = wid / MB, cb = wid - rb * MB;
+        const bool mine = wid < MB * MB;
+        if (mine) {
+            product(X + rb * NS * MU_STEP, X + cb * NS * MU_STEP, NS, acc);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = acc[4 * q + k] * st.gram[it].f_acc;
+                mu_put<NP>(A + mu_block_at(cb, KS, rb * 32, q, lane), v);
+            }
+        }
+        __syncthreads();
+        // B = b A + c A^2, over A
+        float v4[4][4];
+        if (mine) {
+            product(A + rb * KS * MU_STEP, A + cb * KS * MU_STEP, KS, acc);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                mu_get<NP>(A + mu_block_at(cb, KS, rb * 32, q, lane), v4[q]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v4[q][k] = acc[4 * q + k] * st.poly[it].f_acc + v4[q][k] * st.poly[it].f_add;
+            }
+        }
+        __syncthreads();
+        if (mine) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) mu_put<NP>(A + mu_block_at(cb, KS, rb * 32, q, lane), v4[q]);
+        }
+        __syncthreads();
+        // X <- a X + B X
+        mu_acc y[MU_SMALL_BLOCKS];
+#pragma unroll
+        for (int b = 0; b < MU_SMALL_BLOCKS; ++b) {
+            const int id = wid + b * (MU_SMALL_NT / 64);
+            if (id < MB * NB) {
+                const int nb = id / MB, mb = id - nb * MB;
+                zero(y[b]);
+                for (int ks = 0; ks < KS; ++ks) {
+                    mu_h8 r[NP], c[NP];
+#pragma unroll
+                    for (int s = 0; s < NP; ++s) {
+                        c[s] = *reinterpret_cast<const mu_h8*>(A + (mb * KS + ks) * MU_STEP + s * MU_FRAG + ln.direct);
+                        // the two n steps of a block are 2 KiB apart here, not 512 bytes
+                        const char* t = X + ((ks >> 1) * NS + nb * 2) * MU_STEP + s * MU_FRAG + (ks & 1) * 512 +
+                                        ((lane >> 4) & 1) * (MU_STEP - 512);
+                        r[s] = mu_tr(t + ln.tr0, t + ln.tr1);
+                    }
+                    mfma(r, c, y[b]);
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    float x[4];
+                    mu_get<2>(X + mu_block_at(mb, NS, nb * 32, q, lane), x);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) y[b][4 * q + k] = y[b][4 * q + k] * st.step[it].f_acc + x[k] * st.step[it].f_add;
+                }
+            }
+        }
+        __syncthreads();
+        const bool last = it + 1 == st.steps;
+#pragma unroll
+        for (int b = 0; b < MU_SMALL_BLOCKS; ++b) {
+            const int id = wid + b * (MU_SMALL_NT / 64);
+            if (id < MB * NB) {
+                const int nb = id / MB, mb = id - nb * MB;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    float v[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[k] = y[b][4 * q + k];
+                    if (!last) {
+                        mu_put<2>(X + mu_block_at(mb, NS, nb * 32, q, lane), v);
+                    } else {
+                        const int m = mb * 32 + (lane & 31), n = nb * 32 + 8 * q + 4 * h;
+                        if (m < ge.m) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                if (n + k < ge.n)
+                                    mu_finish(out, ge.trans ? (long)(n + k) * ge.m + m : (long)m * ge.n + n + k, v[k], decay,
+                                              ptrs.lr_scale[e], is_step != 0);
+                        }
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------
+struct MuCoef { int steps; float a, b, c, eps; };
+
+// Power-of-two scales of the iterates.  s_k bounds the singular values of X_k: s_0 = 1 and s_{k+1} is the largest
+// |s (a + b s^2 + c s^4)| on [0, s_k] (its ends and the roots of the derivative).  Entries of X are at most s_k,
+// those of A at most s_k^2, those of B at most the largest |b t + c t^2| on [0, s_k^2]; a factor of two is kept for rounding.
+// Returns false where a bound passes 256: the iteration would leave what two fp16 parts hold.
+static bool mu_scales(const MuCoef& co, MuSteps& st, float& x0_scale) {
+    const double a = co.a, b = co.b, c = co.c;
+    double s = 1.0;
+    st.steps = co.steps;
+    auto scale = [](double bound) { return std::exp2(std::floor(std::log2(32768.0 / std::max(bound, 1e-3)))); };
+    double sx = scale(s);
+    x0_scale = (float)sx;
+    for (int k = 0; k < co.steps; ++k) {
+        const double top = s * s;
+        double pb = std::fabs(b * top + c * top * top), next = std::fabs(s * (a + b * top + c * top * top));
+        if (c != 0.0) {
+            const double t = -b / (2 * c);
+            if (t > 0 && t < top) pb = std::max(pb, std::fabs(b * t + c * t * t));
+        }
+        double roots[2];
+        int nr = 0;
+        if (c != 0.0) {
+            const double d = 9 * b * b - 20 * a * c;
+            if (d >= 0) {
+                roots[nr++] = (-3 * b + std::sqrt(d)) / (10 * c);
+                roots[nr++] = (-3 * b - std::sqrt(d)) / (10 * c);
+            }
+        } else if (b != 0.0) {
+            roots[nr++] = -a / (3 * b);
+        }
+        for (int i = 0; i < nr; ++i)
+            if (roots[i] > 0 && roots[i] < top) {
+                const double r = std::sqrt(roots[i]);
+                next = std::max(next, std::fabs(r * (a + b * roots[i] + c * roots[i] * roots[i])));
+            }
+        if (!(top <= 256 && pb <= 256 && next <= 256)) return false;
+        const double sa = scale(top), sb = scale(pb), sn = scale(next);
+        const bool last = k + 1 == co.steps;
+        st.gram[k] = {(float)(sa / (sx * sx)), 0.0f};
+        st.poly[k] = {(float)(c * sb / (sa * sa)), (float)(b * sb / sa)};
+        st.step[k] = {(float)((last ? 1.0 : sn) / (sb * sx)), (float)(a * (last ? 1.0 : sn) / sx)};
+        sx = sn;
+        s = next;
+    }
+    return true;
+}
+
+struct MuJob {                                   // one shape: `count` matrices behind one pointer each
+    long rows, cols, count;
+    void* p;
+    const void* g;
+    float* mom;
+    float lr_scale;
+};
+
+static long mu_up(long v, long t) { return (v + t - 1) / t * t; }
+static bool mu_small(const MuJob& j) {
+    const long m = mu_up(std::min(j.rows, j.cols), 32), n = mu_up(std::max(j.rows, j.cols), 32);
+    return m <= 128 && n <= MU_SMALL_ENTRIES && m * n + m * m <= MU_SMALL_ENTRIES;
+}
+
+constexpr int MU_TARGET_WGS = 512;               // two workgroups per CU: what the splits of X X^T aim at
+constexpr long MU_PASS_BYTES = 1L << 30;         // workspace beyond which a batch is run in several passes
+constexpr long MU_MAX_SIDE = 65536, MU_MAX_LONG = 1L << 24, MU_MAX_ENTRIES = 1L << 36;
+
+static bool mu_shape_ok(long rows, long cols) {
+    const long m = std::min(rows, cols), n = std::max(rows, cols);
+    return m >= 1 && m <= MU_MAX_SIDE && n <= MU_MAX_LONG && m * n <= MU_MAX_ENTRIES;
+}
+
+// The matrices of one pass that take the tiled kernels: at most MU_MAX shapes.
+struct MuPlan {
+    int tile, n;
+    MuGeo geo[MU_MAX];
+    long norm_blocks, bytes;
+};
+
+// 128 x 128 output tiles where there are enough of them for every CU, 64 x 64 where there are not
+static void mu_plan(const MuJob* jobs, int n, MuPlan& pl) {
+    long t128 = 0;
+    for (int i = 0; i < n; ++i) {
+        const long m = std::min(jobs[i].rows, jobs[i].cols), c = std::max(jobs[i].rows, jobs[i].cols);
+        t128 += jobs[i].count * (mu_up(m, 128) / 128) * (mu_up(c, 128) / 128);
+    }
+    const int tile = t128 >= 256 ? 128 : 64;
+    pl.tile = tile;
+    pl.n = n;
+    long work = 0;
+    for (int i = 0; i < n; ++i) {
+        MuGeo& g = pl.geo[i];
+        g.m = (int)std::min(jobs[i].rows, jobs[i].cols);
+        g.n = (int)std::max(jobs[i].rows, jobs[i].cols);
+        g.mp = (int)mu_up(g.m, tile);
+        g.np = (int)mu_up(g.n, tile);
+        g.trans = jobs[i].rows > jobs[i].cols;
+        g.count = (int)jobs[i].count;
+        work += jobs[i].count * mu_tri(g.mp / tile) * (g.np / 16);
+    }
+    // k steps per workgroup of X X^T so that all of them together fill the chip, no fewer than 16
+    const long target = std::max(16L, (work + MU_TARGET_WGS - 1) / MU_TARGET_WGS);
+    pl.norm_blocks = 0;
+    for (int i = 0; i < n; ++i) {
+        MuGeo& g = pl.geo[i];
+        const long ks = g.np / 16;
+        const long s = std::max(1L, (ks + target / 2) / target);
+        g.kper = (int)((ks + s - 1) / s);
+        g.splits = (int)((ks + g.kper - 1) / g.kper);
+        pl.norm_blocks += jobs[i].count * (((long)g.m * g.n + MU_NORM_BLOCK - 1) / MU_NORM_BLOCK);
+    }
+    pl.bytes = mu_up(pl.norm_blocks * 8, 1024);
+    for (int i = 0; i < n; ++i) {
+        pl.geo[i].off = pl.bytes;
+        pl.bytes += jobs[i].count * (tile == 128 ? mu_matrix_bytes<128>(pl.geo[i]) : mu_matrix_bytes<64>(pl.geo[i]));
+    }
+}
+
+struct MuRun {                                   // what the launches of a call share
+    MuCoef co;
+    MuSteps st;
+    float x0_scale, decay;
+    MuMom mm;
+    int is_step;
+    hipStream_t stream;
+};
+
+static void mu_pointers(const MuJob* jobs, int n, MuPtrs& pt) {
+    for (int i = 0; i < MU_MAX; ++i) {
+        pt.p[i] = i < n ? jobs[i].p : nullptr;
+        pt.g[i] = i < n ? jobs[i].g : nullptr;
+        pt.mom[i] = i < n ? jobs[i].mom : nullptr;
+        pt.lr_scale[i] = i < n ? jobs[i].lr_scale : 0.0f;
+    }
+}
+
+// first workgroup of each entry, and their number (0: more than a grid holds)
+template <typename F>
+static int mu_starts(const MuPlan& pl, int* start, F per_matrix) {
+    long at = 0;
+    for (int i = 0; i <= MU_MAX; ++i) {
+        start[i] = i <= pl.n ? (int)at : INT_MAX;
+        if (i < pl.n) at += pl.geo[i].count * per_matrix(pl.geo[i]);
+        if (at > (1L << 30)) return 0;
+    }
+    for (int i = pl.n; i <= MU_MAX; ++i) start[i] = INT_MAX;
+    return (int)at;
+}
+
+template <typename T, int TERMS>
+static int mu_run_small(const MuJob* jobs, int n, const MuRun& r) {
+    MuTab tab;
+    MuPtrs pt;
+    mu_pointers(jobs, n, pt);
+    tab.n = n;
+    long at = 0, most = 0;
+    for (int i = 0; i <= MU_MAX; ++i) tab.start[i] = INT_MAX;
+    for (int i = 0; i < n; ++i) {
+        MuGeo& g = tab.e[i];
+        g.off = 0;
+        g.m = (int)std::min(jobs[i].rows, jobs[i].cols);
+        g.n = (int)std::max(jobs[i].rows, jobs[i].cols);
+        g.mp = (int)mu_up(g.m, 32);
+        g.np = (int)mu_up(g.n, 32);
+        g.trans = jobs[i].rows > jobs[i].cols;
+        g.splits = g.kper = 1;
+        g.count = (int)jobs[i].count;
+        tab.start[i] = (int)at;
+        at += jobs[i].count;
+        most = std::max(most, 4L * g.mp * (g.np + g.mp));
+        MV_REQUIRE(at <= (1L << 30), E_SHAPE, "mdnvae_orthogonalize: too many matrices for one launch");
+    }
+    auto kern = mu_small_kernel<T, TERMS>;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                             4 * MU_SMALL_ENTRIES);
+    MV_REQUIRE(e == hipSuccess, (int)e, "mu_small_kernel: cannot raise the LDS limit: %s", hipGetErrorString(e));
+    hipLaunchKernelGGL(kern, dim3((unsigned)at), dim3(MU_SMALL_NT), (size_t)most, r.stream, tab, pt, r.mm, r.co.eps, r.x0_scale, r.st,
+                       r.decay, r.is_step);
+    MV_LAUNCH_CHECK("mu_small_kernel");
+    return 0;
+}
+
+template <typename T, int TERMS, int TILE>
+static int mu_run_tiled(const MuJob* jobs, const MuPlan& pl, const MuRun& r, char* ws) {
+    MuPtrs pt;
+    mu_pointers(jobs, pl.n, pt);
+    MuTab tab;
+    tab.n = pl.n;
+    for (int i = 0; i < MU_MAX; ++i) tab.e[i] = pl.geo[i < pl.n ? i : 0];
+    MuStarts norm;
+    const int n_norm = mu_starts(pl, norm.s, [](const MuGeo& g) { return ((long)g.m * g.n + MU_NORM_BLOCK - 1) / MU_NORM_BLOCK; });
+    MuTab tsplit = tab, tgram = tab, tpoly = tab, tstep = tab;
+    const int n_split = mu_starts(pl, tsplit.start, [](const MuGeo& g) { return (long)(g.mp / 32) * (g.np / 64); });
+    const int n_gram = mu_starts(pl, tgram.start, [](const MuGeo& g) { return mu_tri(g.mp / TILE) * g.splits; });
+    const int n_poly = mu_starts(pl, tpoly.start, [](const MuGeo& g) { return mu_tri(g.mp / TILE); });
+    const int n_step = mu_starts(pl, tstep.start, [](const MuGeo& g) { return (long)(g.mp / TILE) * (g.np / TILE); });
+    MV_REQUIRE(n_norm && n_split && n_gram && n_poly && n_step, E_SHAPE, "mdnvae_orthogonalize: too many tiles for one launch");
+    bool split = false;
+    for (int i = 0; i < pl.n; ++i) split = split || pl.geo[i].splits > 1;
+    double* partial = reinterpret_cast<double*>(ws);
+    MuTab tnorm = tab;
+    for (int i = 0; i <= MU_MAX; ++i) tnorm.start[i] = norm.s[i];
+    hipLaunchKernelGGL((mu_norm_kernel<T>), dim3(n_norm), dim3(256), 0, r.stream, tnorm, pt, r.mm, partial);
+    MV_LAUNCH_CHECK("mu_norm_kernel");
+    hipLaunchKernelGGL((mu_split_kernel<T>), dim3(n_split), dim3(256), 0, r.stream, tsplit, norm, pt, r.mm, r.co.eps, r.x0_scale,
+                       (const double*)partial, ws, TILE == 128 ? 1 : 0);
+    MV_LAUNCH_CHECK("mu_split_kernel");
+    constexpr size_t lds = (size_t)4 * 2 * (TILE / 32) * (TERMS == 3 ? 2 : 1) * MU_FRAG;
+    static_assert(lds <= 64 * 1024 && lds >= 4 * 4096, "the ring fits the default LDS limit and holds the mirror's blocks");
+    auto grid = [](int n) { return dim3((unsigned)((n + 7) / 8 * 8)); };
+    for (int it = 0; it < r.st.steps; ++it) {
+        const int ping = it & 1;
+        hipLaunchKernelGGL((mu_sym_kernel<TILE, TERMS, MU_GRAM>), grid(n_gram), dim3(256), lds, r.stream, tgram, n_gram, ws, ping,
+                           r.st.gram[it]);
+        MV_LAUNCH_CHECK("mu_sym_kernel");
+        if (split) {
+            hipLaunchKernelGGL((mu_reduce_kernel<TILE, TERMS>), dim3(n_poly), dim3(256), 0, r.stream, tpoly, ws, r.st.gram[it]);
+            MV_LAUNCH_CHECK("mu_reduce_kernel");
+        }
+        hipLaunchKernelGGL((mu_sym_kernel<TILE, TERMS, MU_POLY>), grid(n_poly), dim3(256), lds, r.stream, tpoly, n_poly, ws, ping,
+                           r.st.poly[it]);
+        MV_LAUNCH_CHECK("mu_sym_kernel");
+        if (it + 1 < r.st.steps)
+            hipLaunchKernelGGL((mu_step_kernel<T, TILE, TERMS, false>), grid(n_step), dim3(256), lds, r.stream, tstep, n_step, pt, ws,
+                               ping, r.st.step[it], r.decay, r.is_step);
+        else
+            hipLaunchKernelGGL((mu_step_kernel<T, TILE, TERMS, true>), grid(n_step), dim3(256), lds, r.stream, tstep, n_step, pt, ws,
+                               ping, r.st.step[it], r.decay, r.is_step);
+        MV_LAUNCH_CHECK("mu_step_kernel");
+    }
+    return 0;
+}
+
+template <typename T, int TERMS>
+static int mu_run(const MuJob* jobs, int n, bool small, const MuRun& r, char* ws) {
+    if (n == 0) return 0;
+    if (small) return mu_run_small<T, TERMS>(jobs, n, r);
+    MuPlan pl;
+    mu_plan(jobs, n, pl);
+    return pl.tile == 128 ? mu_run_tiled<T, TERMS, 128>(jobs, pl, r, ws) : mu_run_tiled<T, TERMS, 64>(jobs, pl, r, ws);
+}
+static int mu_dispatch(const MuJob* jobs, int n, bool small, int dtype, int terms, const MuRun& r, char* ws) {
+    if (dtype == MDNVAE_F32)
+        return terms == 3 ? mu_run<float, 3>(jobs, n, small, r, ws) : mu_run<float, 1>(jobs, n, small, r, ws);
+    return terms == 3 ? mu_run<__bf16, 3>(jobs, n, small, r, ws) : mu_run<__bf16, 1>(jobs, n, small, r, ws);
+}
+
+// matrices of a batch that go through one pass
+static long mu_batch_per_pass(long batch, long rows, long cols) {
+    MuJob j = {rows, cols, 1, nullptr, nullptr, nullptr, 0.0f};
+    if (mu_small(j)) return batch;
+    MuPlan pl;
+    mu_plan(&j, 1, pl);                           // what one matrix takes alone: more splits than in company, if anything
+    return std::max(1L, std::min(batch, MU_PASS_BYTES / std::max(1L, pl.bytes)));
+}
+
+static int mu_check(const char* who, int dtype, int terms, int steps, float a, float b, float c, float eps, MuRun& r) {
+    MV_REQUIRE(dtype == MDNVAE_F32 || dtype == MDNVAE_BF16, E_ARG, "%s: unknown element type %d", who, dtype);
+    MV_REQUIRE(terms == 1 || terms == 3, E_ARG, "%s: products have 1 or 3 terms (got %d)", who, terms);
+    MV_REQUIRE(steps >= 1 && steps <= MDNVAE_MUON_MAX_STEPS, E_ARG, "%s: steps = %d outside [1, %d]", who, steps, MDNVAE_MUON_MAX_STEPS);
+    MV_REQUIRE(eps > 0.0f && std::isfinite(eps), E_ARG, "%s: eps must be positive and finite", who);
+    MV_REQUIRE(std::isfinite(a) && std::isfinite(b) && std::isfinite(c), E_ARG, "%s: coefficients must be finite", who);
+    r.co = {steps, a, b, c, eps};
+    MV_REQUIRE(mu_scales(r.co, r.st, r.x0_scale), E_ARG,
+               "%s: with these coefficients the iteration may leave [-256, 256] (singular values start in [0, 1])", who);
+    return 0;
+}
+
+}  // namespace mdnvae
+using namespace mdnvae;
+
+extern "C" size_t mdnvae_orthogonalize_workspace_bytes(long batch, long rows, long cols) {
+    if (batch < 1 || !mu_shape_ok(rows, cols)) return 0;
+    const long per = mu_batch_per_pass(batch, rows, cols), rest = batch % per;
+    MuJob j = {rows, cols, per, nullptr, nullptr, nullptr, 0.0f};
+    if (mu_small(j)) return 0;
+    MuPlan pl;
+    mu_plan(&j, 1, pl);
+    long bytes = pl.bytes;
+    if (rest) {                                   // the last pass plans for itself
+        j.count = rest;
+        mu_plan(&j, 1, pl);
+        bytes = std::max(bytes, pl.bytes);
+    }
+    return (size_t)bytes;
+}
+
+extern "C" int mdnvae_orthogonalize(const void* x, void* out, long batch, long rows, long cols, int dtype, int steps, float a, float b,
+                                    float c, float eps, int terms, void* workspace, size_t workspace_bytes, void* stream) {
+    MV_REQUIRE(batch >= 0 && rows >= 0 && cols >= 0, E_ARG, "mdnvae_orthogonalize: negative size");
+    MuRun r = {};
+    const int bad = mu_check("mdnvae_orthogonalize", dtype, terms, steps, a, b, c, eps, r);
+    if (bad) return bad;
+    if (batch == 0 || rows == 0 || cols == 0) return 0;
+    MV_REQUIRE(mu_shape_ok(rows, cols) && batch <= (1L << 30), E_SHAPE, "mdnvae_orthogonalize: %ld x [%ld, %ld] is larger than the kernels index", batch,
+               rows, cols);
+    MV_REQUIRE(x && out, E_ARG, "mdnvae_orthogonalize: null pointer");
+    const size_t need = mdnvae_orthogonalize_workspace_bytes(batch, rows, cols);
+    MV_REQUIRE(workspace_bytes >= need && (workspace || need == 0), E_ARG, "mdnvae_orthogonalize: workspace of %zu bytes, %zu are needed",
+               workspace_bytes, need);
+    MV_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, E_ALIGN, "mdnvae_orthogonalize: workspace must be 256-byte aligned");
+    r.stream = (hipStream_t)stream;
+    r.decay = 0.0f;
+    r.is_step = 0;
+    const long per = mu_batch_per_pass(batch, rows, cols), size = dtype == MDNVAE_F32 ? 4 : 2;
+    for (long at = 0; at < batch; at += per) {
+        MuJob j = {rows, cols, std::min(per, batch - at), static_cast<char*>(out) + at * rows * cols * size,
+                   static_cast<const char*>(x) + at * rows * cols * size, nullptr, 0.0f};
+        const int rc = mu_dispatch(&j, 1, mu_small(j), dtype, terms, r, static_cast<char*>(workspace));
+        if (rc) return rc;
+    }
+    return 0;
+}
+
+// The matrices of a step in order, `f(jobs, n, small)` for each group of up to MU_MAX that is launched together; stops at the
+// first result that is not 0.
+template <typename F>
+static int mu_groups(const long* rows, const long* cols, int count, F f) {
+    for (int pass = 0; pass < 2; ++pass) {
+        MuJob jobs[MU_MAX];
+        int index[MU_MAX], n = 0;
+        for (int i = 0; i < count; ++i) {
+            if (rows[i] == 0 || cols[i] == 0) continue;
+            MuJob j = {rows[i], cols[i], 1, nullptr, nullptr, nullptr, 0.0f};
+            if (mu_small(j) != (pass == 1)) continue;
+            jobs[n] = j;
+            index[n++] = i;
+            if (n == MU_MAX) {
+                const int rc = f(jobs, index, n, pass == 1);
+                if (rc) return rc;
+                n = 0;
+            }
+        }
+        if (n) {
+            const int rc = f(jobs, index, n, pass == 1);
+            if (rc) return rc;
+        }
+    }
+    return 0;
+}
+
+extern "C" size_t mdnvae_muon_workspace_bytes(const long* rows, const long* cols, int count) {
+    if (count < 1 || !rows || !cols) return 0;
+    for (int i = 0; i < count; ++i)
+        if (rows[i] < 0 || cols[i] < 0 || (rows[i] > 0 && cols[i] > 0 && !mu_shape_ok(rows[i], cols[i]))) return 0;
+    long most = 0;
+    mu_groups(rows, cols, count, [&](MuJob* jobs, const int*, int n, bool small) {
+        if (!small) {
+            MuPlan pl;
+            mu_plan(jobs, n, pl);
+            most = std::max(most, pl.bytes);
+        }
+        return 0;
+    });
+    return (size_t)most;
+}
+
+extern "C" int mdnvae_muon_step(void* const* params, const void* const* grads, float* const* momenta, const long* rows, const long* cols,
+                                int count, int dtype, float lr, float momentum, int nesterov, float weight_decay, int scale_mode,
+                                int steps, float a, float b, float c, float eps, int terms, void* workspace, size_t workspace_bytes,
+                                void* stream) {
+    MV_REQUIRE(count >= 0, E_ARG, "mdnvae_muon_step: negative count");
+    MuRun r = {};
+    const int bad = mu_check("mdnvae_muon_step", dtype, terms, steps, a, b, c, eps, r);
+    if (bad) return bad;
+    MV_REQUIRE(std::isfinite(lr) && std::isfinite(weight_decay) && momentum >= 0.0f && momentum < 1.0f, E_ARG,
+               "mdnvae_muon_step: lr and weight_decay must be finite, momentum in [0, 1)");
+    MV_REQUIRE(scale_mode >= MDNVAE_MUON_SCALE_NONE && scale_mode <= MDNVAE_MUON_SCALE_RMS, E_ARG, "mdnvae_muon_step: unknown scale mode %d",
+               scale_mode);
+    if (count == 0) return 0;
+    MV_REQUIRE(params && grads && momenta && rows && cols, E_ARG, "mdnvae_muon_step: null pointer");
+    for (int i = 0; i < count; ++i) {
+        MV_REQUIRE(rows[i] >= 0 && cols[i] >= 0, E_ARG, "mdnvae_muon_step: negative size of matrix %d", i);
+        if (rows[i] == 0 || cols[i] == 0) continue;
+        MV_REQUIRE(mu_shape_ok(rows[i], cols[i]), E_SHAPE, "mdnvae_muon_step: matrix %d [%ld, %ld] is larger than the kernels index", i, rows[i],
+                   cols[i]);
+        MV_REQUIRE(params[i] && grads[i] && momenta[i], E_ARG, "mdnvae_muon_step: null pointer of matrix %d", i);
+    }
+    const size_t need = mdnvae_muon_workspace_bytes(rows, cols, count);
+    MV_REQUIRE(workspace_bytes >= need && (workspace || need == 0), E_ARG, "mdnvae_muon_step: workspace of %zu bytes, %zu are needed",
+               workspace_bytes, need);
+    MV_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, E_ALIGN, "mdnvae_muon_step: workspace must be 256-byte aligned");
+    r.stream = (hipStream_t)stream;
+    r.decay = (float)(1.0 - (double)lr * (double)weight_decay);
+    r.mm = {momentum, nesterov};
+    r.is_step = 1;
+    return mu_groups(rows, cols, count, [&](MuJob* jobs, const int* index, int n, bool small) {
+        for (int k = 0; k < n; ++k) {
+            const int i = index[k];
+            const double ro = (double)rows[i], co = (double)cols[i];
+            const double s = scale_mode == MDNVAE_MUON_SCALE_SHAPE ? std::sqrt(std::max(1.0, ro / co))
+                             : scale_mode == MDNVAE_MUON_SCALE_RMS ? 0.2 * std::sqrt(std::max(ro, co)) : 1.0;
+            jobs[k].p = params[i];
+            jobs[k].g = grads[i];
+            jobs[k].mom = momenta[i];
+            jobs[k].lr_scale = (float)((double)lr * s);
+        }
+        return mu_dispatch(jobs, n, small, dtype, terms, r, static_cast<char*>(workspace));
+    });
+}

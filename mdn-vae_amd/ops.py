@@ -1,6 +1,7 @@
 """Autograd wrappers over the C ABI: each op's forward and backward are hand-written HIP
 kernels; nothing here computes on the host or falls back to eager PyTorch arithmetic."""
 import contextlib
+import ctypes
 
 import torch
 
@@ -1970,3 +1971,111 @@ def softmax_rows(logits):
         m = logits.max(dim=1, keepdim=True).values
         e = exp(logits - m)
         return e / e.sum(dim=1, keepdim=True)
+
+
+# ---------------------------------------------------------------------------------------
+# orthogonalised updates (csrc/muon.hip)
+# ---------------------------------------------------------------------------------------
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)      # steep at zero: small singular values reach [0.7, 1.2] in five steps
+ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1}
+UPDATE_SCALES = {None: 0, "shape": 1, "rms": 2}
+
+
+def _element_type(t, name):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
+    if t.dtype not in ELEMENT_TYPES:
+        raise RuntimeError(f"{name}: dtype {t.dtype}, expected torch.float32 or torch.bfloat16")
+    return ELEMENT_TYPES[t.dtype]
+
+
+def _update_terms(arithmetic, dtype):
+    if arithmetic is None:
+        return 3 if dtype == torch.float32 else 1
+    if arithmetic not in ("f16x2", "f16"):
+        raise ValueError(f"arithmetic {arithmetic!r}: 'f16x2' (two fp16 parts per operand) or 'f16' (the high part)")
+    return 3 if arithmetic == "f16x2" else 1
+
+
+def _workspace(nbytes, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def orthogonalize(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, arithmetic=None, out=None):
+    """The nearest thing to an orthogonal matrix that `steps` Newton-Schulz steps reach from each matrix of x [..., m, n]
+    (fp32 or bf16, contiguous): X = x / max(|x|_F, eps), then X <- a X + (b A + c A^2) X with A = X X^T (of the
+    transposed matrix if m > n).  Same shape and type as x; `out` may be given, and may be x.  Not differentiable.
+
+    arithmetic: 'f16x2' (default for fp32) products from two fp16 parts per operand, fp32-level; 'f16' (default for
+    bf16) one product of the high parts, about 1e-3 of the result's norm, a third of the work.
+    A matrix that holds a NaN or an infinity becomes NaN throughout (the others of the batch do not), a zero matrix
+    stays zero.  Coefficients with which a singular value of [0, 1] could pass 256 are refused."""
+    dtype = _element_type(x, "x")
+    if x.dim() < 2:
+        raise RuntimeError(f"orthogonalize: x {tuple(x.shape)} must have at least two dimensions")
+    x = x.detach()
+    xp = ptr(x, "x", x.dtype)
+    if out is None:
+        out = torch.empty_like(x)
+    else:
+        out = out.detach()
+        if out.shape != x.shape or out.device != x.device:
+            raise RuntimeError(f"orthogonalize: out {tuple(out.shape)} on {out.device} must match x {tuple(x.shape)} on {x.device}")
+    op = ptr(out, "out", x.dtype)
+    if x.numel() == 0:
+        return out
+    rows, cols = x.shape[-2:]
+    batch = x.numel() // (rows * cols)
+    a, b, c = (float(v) for v in coefficients)
+    lib = _lib.load()
+    with torch.cuda.device(x.device):
+        ws = _workspace(lib.mdnvae_orthogonalize_workspace_bytes(batch, rows, cols), x.device)
+        call("mdnvae_orthogonalize", xp, op, batch, rows, cols, dtype, int(steps), a, b, c, float(eps),
+             _update_terms(arithmetic, x.dtype), None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), stream())
+    return out
+
+
+def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_decay=0.0, scale="shape", steps=5,
+              coefficients=NS_COEFFICIENTS, eps=1e-7, arithmetic=None):
+    """One optimizer step with orthogonalised updates, in place, for a list of weights of any shapes:
+        M <- momentum M + g;  u = g + momentum M (nesterov) or M;  p <- (1 - lr weight_decay) p - lr s orthogonalize(u)
+    params and grads: fp32 or bf16 tensors (one type for all), momenta: fp32 tensors of the same shapes; contiguous, on
+    one device.  A tensor of more than two dimensions (a convolution's weight) counts as [first, all the others].
+    scale: 'shape' s = sqrt(max(1, rows / cols)), 'rms' s = 0.2 sqrt(max(rows, cols)) (the size of an Adam step), None s = 1.
+    Matrices that fit one workgroup's LDS take one launch together, all the others share each launch of the
+    tiled products.  steps, coefficients, eps, arithmetic: as for `orthogonalize`."""
+    params, grads, momenta = list(params), list(grads), list(momenta)
+    if not len(params) == len(grads) == len(momenta):
+        raise RuntimeError(f"muon_step: {len(params)} parameters, {len(grads)} gradients, {len(momenta)} momenta")
+    if scale not in UPDATE_SCALES:
+        raise ValueError(f"scale {scale!r}: one of {list(UPDATE_SCALES)}")
+    if not params:
+        return
+    dtype, dev = _element_type(params[0], "params[0]"), params[0].device
+    n = len(params)
+    pp, gp, mp = (ctypes.c_void_p * n)(), (ctypes.c_void_p * n)(), (ctypes.c_void_p * n)()
+    rows, cols = (ctypes.c_long * n)(), (ctypes.c_long * n)()
+    spans = []
+    for i, (p, g, m) in enumerate(zip(params, grads, momenta)):
+        if not isinstance(p, torch.Tensor) or p.dim() < 2:
+            raise RuntimeError(f"muon_step: params[{i}] must be a tensor of at least two dimensions")
+        pp[i], gp[i] = ptr(p.detach(), f"params[{i}]", params[0].dtype), ptr(g, f"grads[{i}]", params[0].dtype)
+        mp[i] = ptr(m, f"momenta[{i}]", torch.float32)
+        if g is None or m is None or g.shape != p.shape or m.shape != p.shape:
+            raise RuntimeError(f"muon_step: params[{i}] {tuple(p.shape)} needs a gradient and a momentum of its shape")
+        if p.device != dev or g.device != dev or m.device != dev:
+            raise RuntimeError(f"muon_step: params[{i}], its gradient and its momentum must all be on {dev}")
+        rows[i] = p.shape[0]
+        cols[i] = p.numel() // p.shape[0] if p.numel() else 0
+        if p.numel():
+            spans += [(pp[i], p.numel() * p.element_size()), (mp[i], 4 * m.numel())]
+    spans.sort()
+    if any(a + size > b for (a, size), (b, _) in zip(spans, spans[1:])):
+        raise RuntimeError("muon_step: parameters and momenta must not overlap (is a tensor in the list twice?)")
+    a, b, c = (float(v) for v in coefficients)
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        ws = _workspace(lib.mdnvae_muon_workspace_bytes(rows, cols, n), dev)
+        call("mdnvae_muon_step", pp, gp, mp, rows, cols, n, dtype, float(lr), float(momentum), int(bool(nesterov)), float(weight_decay),
+             UPDATE_SCALES[scale], int(steps), a, b, c, float(eps), _update_terms(arithmetic, params[0].dtype),
+             None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), stream())
