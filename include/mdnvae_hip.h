@@ -727,6 +727,25 @@ int mdnvae_muon_step(void* const* params, const void* const* grads, float* const
                      int count, int dtype, float lr, float momentum, int nesterov, float weight_decay, int scale_mode, int steps,
                      float a, float b, float c, float eps, int terms, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- balance loss of a gate ------------------------------------------------------------------------
+ * For the gate of the trait-gated mixture (no counterpart in the reference): logits [T][E], fp32 or bf16 (`dtype`),
+ * 1 <= E <= 1024, 1 <= top_k <= E; valid [T] bytes or NULL (all rows).  p = softmax(logits) of the n valid rows,
+ *     counts[e] = rows with e among their top_k largest logits (ties: the lowest index)
+ *     mean_probs[e] = mean of p_e,   loss = E / (top_k n) sum_e counts[e] mean_probs[e],   n_valid[0] = n
+ *     grad = dloss / dlogits [T][E] in the logits' type, zeros in rows that are not valid; NULL: not wanted
+ * A logit of -inf masks that expert out of that row (p = 0, never counted), a row of nothing else is not valid.  A NaN or
+ * +inf in a valid row gives NaN there (NaN counts as the largest number).  n = 0: zeros.  Logits of rows that are not
+ * valid are never looked at.  Sums in fixed order. */
+size_t mdnvae_gate_balance_workspace_bytes(long T, int E);
+int mdnvae_gate_balance(const void* logits, const unsigned char* valid, long T, int E, int top_k, int dtype, void* workspace,
+                        size_t workspace_bytes, float* loss, int* counts, float* mean_probs, int* n_valid, void* grad,
+                        void* stream);
+/* grad for upstream gradients g_loss [1] (NULL: 1) of the loss and g_mean [E] (NULL: none) of mean_probs, from the
+ * forward pass's counts, mean_probs and n_valid.  counts carry no gradient. */
+int mdnvae_gate_balance_bwd(const void* logits, const unsigned char* valid, long T, int E, int top_k, int dtype,
+                            const int* counts, const float* mean_probs, const int* n_valid, const float* g_loss,
+                            const float* g_mean, void* grad, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -2079,3 +2079,74 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
         call("mdnvae_muon_step", pp, gp, mp, rows, cols, n, dtype, float(lr), float(momentum), int(bool(nesterov)), float(weight_decay),
              UPDATE_SCALES[scale], int(steps), a, b, c, float(eps), _update_terms(arithmetic, params[0].dtype),
              None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), stream())
+
+
+# ---------------------------------------------------------------------------------------
+# balance loss of a gate (csrc/gate.hip)
+# ---------------------------------------------------------------------------------------
+def _gate_call(logits, top_k, valid, want_grad):
+    dtype = _element_type(logits, "logits")
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise RuntimeError(f"gate balance loss: logits {tuple(logits.shape)} must be [rows, experts]")
+    T, E = logits.shape
+    lp, vp, dev = ptr(logits, "logits", logits.dtype), ptr(valid, "valid", torch.bool), logits.device
+    if valid is not None and (valid.shape != (T,) or valid.device != dev):
+        raise RuntimeError(f"gate balance loss: valid {tuple(valid.shape)} on {valid.device} must be [{T}] on {dev}")
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        counts = torch.empty(E, dtype=torch.int32, device=dev)
+        mean_probs = torch.empty(E, dtype=torch.float32, device=dev)
+        n_valid = torch.empty(1, dtype=torch.int32, device=dev)
+        grad = torch.empty_like(logits) if want_grad else None
+        ws = _workspace(lib.mdnvae_gate_balance_workspace_bytes(T, E), dev)
+        call("mdnvae_gate_balance", lp, vp, T, E, int(top_k), dtype, None if ws is None else ws.data_ptr(),
+             0 if ws is None else ws.numel(), loss.data_ptr(), counts.data_ptr(), mean_probs.data_ptr(), n_valid.data_ptr(),
+             None if grad is None else grad.data_ptr(), stream())
+    return loss, counts, mean_probs, n_valid, grad
+
+
+class _GateBalance(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, top_k, valid):
+        loss, counts, mean_probs, n_valid, _ = _gate_call(logits, top_k, valid, False)
+        ctx.save_for_backward(logits, valid, counts, mean_probs, n_valid)
+        ctx.top_k = int(top_k)
+        ctx.mark_non_differentiable(counts)
+        ctx.set_materialize_grads(False)
+        return loss, counts, mean_probs
+
+    @staticmethod
+    def backward(ctx, g_loss, _, g_mean):
+        logits, valid, counts, mean_probs, n_valid = ctx.saved_tensors
+        if g_loss is None and g_mean is None:
+            return None, None, None
+        T, E = logits.shape
+        with torch.cuda.device(logits.device):
+            if g_loss is None:
+                g_loss = torch.zeros((), dtype=torch.float32, device=logits.device)
+            g_loss, g_mean = _c(g_loss), None if g_mean is None else _c(g_mean)
+            grad = torch.empty_like(logits)
+            call("mdnvae_gate_balance_bwd", logits.data_ptr(), ptr(valid, "valid", torch.bool), T, E, ctx.top_k, ELEMENT_TYPES[logits.dtype],
+                 counts.data_ptr(), mean_probs.data_ptr(), n_valid.data_ptr(), ptr(g_loss, "g_loss"), ptr(g_mean, "g_mean"),
+                 grad.data_ptr(), stream())
+        return grad, None, None
+
+
+def gate_balance_loss(logits, top_k=1, valid=None):
+    """How evenly a gate spreads the rows of a batch over its experts (components): (loss, counts, mean_probs).
+    logits [rows, experts] fp32 or bf16, contiguous; valid [rows] bool (None: all).  With p = softmax(logits):
+        counts[e] (int32) = valid rows that have e among their top_k largest logits (ties: the lowest index)
+        mean_probs[e] (fp32) = mean of p_e over the n valid rows
+        loss = experts / (top_k n) * sum_e counts[e] mean_probs[e]
+    which is 1 where the rows spread evenly and grows as they agree.  loss and mean_probs are differentiable with respect to
+    logits, counts are not.  A logit of -inf masks that expert out of its row (never counted), a row of nothing else is
+    not valid; NaN counts as the largest number and shows in the loss.  What rows that are not valid hold is never
+    looked at, and their gradient is zero.  No valid row: zeros."""
+    return _GateBalance.apply(logits, top_k, valid)
+
+
+def gate_balance_loss_and_grads(logits, top_k=1, valid=None):
+    """The same with the gradient of the loss (upstream 1) from the one call: (loss, counts, mean_probs, grad_logits)."""
+    loss, counts, mean_probs, _, grad = _gate_call(logits.detach() if isinstance(logits, torch.Tensor) else logits, top_k, valid, True)
+    return loss, counts, mean_probs, grad
