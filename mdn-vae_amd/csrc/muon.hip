@@ -15,10 +15,10 @@
 // of the high parts only (a X still from both): 0.3e-3 .. 1.9e-3 of the norm, next to 1.7e-3 of the result's own rounding.
 //
 // Layout.  A matrix [R][K] lives as tiles of 32 rows x 16 k, [R/32][K/16][part 2][32 rows x 32 bytes], the two
-// 16-byte halves of a row swapped where (row & 4): a 1 KiB tile is one LDS-DMA piece, a matrix operand with k along
+// 16-byte halves of a row swapped where (row & 8): a 1 KiB tile is one LDS-DMA piece, a matrix operand with k along
 // the row is one ds_read_b128 per lane, and the operand with k down the column (X in B X) is two transposing
-// ds_read_b64_tr_b16 per lane of the same tile - so X needs no second, transposed copy.  Both read whole 128-byte
-// groups of banks.
+// ds_read_b64_tr_b16 per lane of the same tile - so X needs no second, transposed copy.  With that swap the 16 lanes that
+// a ds_read_b128 serves per clock fall on all 64 banks (4.1 clk per wave; 8.0 without it or with (row & 4)).
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -37,7 +37,7 @@ typedef float mu_f4 __attribute__((ext_vector_type(4)));
 constexpr int MU_FRAG = 1024;            // one part of one 32 x 16 tile
 constexpr int MU_STEP = 2 * MU_FRAG;     // both parts
 constexpr int MU_MAX = 32;               // table entries per launch (kernel arguments stay under 4 KB)
-constexpr int MU_NORM_BLOCK = 16384;     // entries of G per workgroup of the norm pass
+constexpr int MU_NORM_BLOCK = 8192;     // entries of G per workgroup of the norm pass
 
 #define MU_GLOBAL_PTR(p) ((const __attribute__((address_space(1))) void*)(p))
 #define MU_LDS_PTR(p) ((__attribute__((address_space(3))) void*)(p))
@@ -113,10 +113,34 @@ __global__ __launch_bounds__(256) void mu_norm_kernel(MuTab tab, MuPtrs ptrs, Mu
     float* mom = ptrs.mom[e];
     const long lo = blk * MU_NORM_BLOCK, hi = min(len, lo + MU_NORM_BLOCK);
     double s = 0.0;
-#pragma unroll 8
-    for (long i = lo + threadIdx.x; i < hi; i += 256) {
-        const double u = (double)mu_update(g, mom, i, mm, true);
-        s += u * u;
+    typedef T vec __attribute__((ext_vector_type(4)));
+    if (hi - lo == MU_NORM_BLOCK && ((reinterpret_cast<uintptr_t>(g + lo) & (4 * sizeof(T) - 1)) | (reinterpret_cast<uintptr_t>(mom) & 15)) == 0) {
+        constexpr int V = MU_NORM_BLOCK / 1024;            // four entries per access, all loads ahead of the stores
+        vec gv[V];
+        mu_f4 mv[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) gv[i] = *reinterpret_cast<const vec*>(g + lo + (i * 256 + threadIdx.x) * 4);
+        if (mom) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) mv[i] = *reinterpret_cast<const mu_f4*>(mom + lo + (i * 256 + threadIdx.x) * 4);
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            mu_f4 out;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float gk = (float)gv[i][k];
+                out[k] = mom ? mm.mu * mv[i][k] + gk : gk;
+                const double u = mom && mm.nesterov ? (double)(gk + mm.mu * out[k]) : (double)out[k];
+                s += u * u;
+            }
+            if (mom) *reinterpret_cast<mu_f4*>(mom + lo + (i * 256 + threadIdx.x) * 4) = out;
+        }
+    } else {
+        for (long i = lo + threadIdx.x; i < hi; i += 256) {
+            const double u = (double)mu_update(g, mom, i, mm, true);
+            s += u * u;
+        }
     }
     s = block_sum<256, double>(s, red);
     if (threadIdx.x == 0) partial[blockIdx.x] = s;
@@ -135,7 +159,7 @@ __device__ __forceinline__ void mu_parts(float t, _Float16& h, _Float16& l) {
 }
 
 // byte offset of (row, 16-byte half) inside a tile
-__device__ __forceinline__ int mu_at(int row, int half) { return row * 32 + ((half ^ ((row >> 2) & 1)) << 4); }
+__device__ __forceinline__ int mu_at(int row, int half) { return row * 32 + ((half ^ ((row >> 3) & 1)) << 4); }
 
 // ---- split pass: X_0 in parts; one workgroup = 32 rows x 64 columns of X, through LDS so that lanes run along the
 // caller's contiguous dimension ----------------------------------------------------------------------------------------
@@ -199,39 +223,82 @@ struct MuScale {
     float f_add;       // what the tile already there (A in POLY, X in STEP) is multiplied with
 };
 
-__device__ __forceinline__ mu_h8 mu_tr(const char* p0, const char* p1) {
-    const mu_s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) mu_s4*)(p0));
-    const mu_s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) mu_s4*)(p1));
+// lane offsets of the two ways to read an operand of 32 x 16 out of LDS
+struct MuLane {
+    int direct;        // rows of the tile are operand rows
+    int tr;            // columns of two adjacent 16-row half tiles (512 bytes each) are operand rows: k 0..3 of the lane's
+};                     // eight here, k 4..7 four rows (128 bytes) further on
+__device__ __forceinline__ MuLane mu_lane(int lane) {
+    MuLane o;
+    o.direct = mu_at(lane & 31, lane >> 5);
+    const int g = lane >> 4, n16 = g & 1, h = g >> 1, r = (lane & 15) >> 2, ch = lane & 3;
+    o.tr = n16 * 512 + (8 * h + r) * 32 + (((ch >> 1) ^ h) << 4) + (ch & 1) * 8;
+    return o;
+}
+__device__ __forceinline__ mu_h8 mu_join(mu_s4 a, mu_s4 b) {
     mu_s8 f;
     f[0] = a[0]; f[1] = a[1]; f[2] = a[2]; f[3] = a[3];
     f[4] = b[0]; f[5] = b[1]; f[6] = b[2]; f[7] = b[3];
     return __builtin_bit_cast(mu_h8, f);
 }
-
-// lane offsets of the two ways to read an operand of 32 x 16 out of LDS
-struct MuLane {
-    int direct;        // rows of the tile are operand rows
-    int tr0, tr1;      // columns of two adjacent 16-row half tiles (512 bytes each) are operand rows
-};
-__device__ __forceinline__ MuLane mu_lane(int lane) {
-    MuLane o;
-    o.direct = mu_at(lane & 31, lane >> 5);
-    const int g = lane >> 4, n16 = g & 1, h = g >> 1, r = (lane & 15) >> 2, ch = lane & 3;
-    o.tr0 = n16 * 512 + (8 * h + r) * 32 + ((ch >> 1) << 4) + (ch & 1) * 8;
-    o.tr1 = n16 * 512 + (8 * h + 4 + r) * 32 + (((ch >> 1) ^ 1) << 4) + (ch & 1) * 8;
-    return o;
+__device__ __forceinline__ mu_h8 mu_tr(const char* p) {
+    return mu_join(__builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) mu_s4*)(p)),
+                   __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) mu_s4*)(p + 128)));
+}
+// N operands 1 KiB apart.  In the products' loop the builtin would make the compiler wait for every LDS-DMA in flight (it
+// cannot tell that they go elsewhere), which takes the ring's depth away: 1.6x the time of a step.  So the reads and their
+// wait are one block of assembly.
+template <int N>
+__device__ __forceinline__ void mu_tr_block(const char* p, mu_h8 (&out)[N]) {
+    const unsigned at = (unsigned)(size_t)(__attribute__((address_space(3))) const char*)(p);
+    mu_s4 a[2 * N];
+    if constexpr (N == 4) {
+        asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:128\n\t"
+                     "ds_read_b64_tr_b16 %2, %8 offset:1024\n\tds_read_b64_tr_b16 %3, %8 offset:1152\n\t"
+                     "ds_read_b64_tr_b16 %4, %8 offset:2048\n\tds_read_b64_tr_b16 %5, %8 offset:2176\n\t"
+                     "ds_read_b64_tr_b16 %6, %8 offset:3072\n\tds_read_b64_tr_b16 %7, %8 offset:3200\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(a[0]), "=&v"(a[1]), "=&v"(a[2]), "=&v"(a[3]), "=&v"(a[4]), "=&v"(a[5]), "=&v"(a[6]), "=&v"(a[7])
+                     : "v"(at)
+                     : "memory");
+    } else if constexpr (N == 2) {
+        asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:128\n\t"
+                     "ds_read_b64_tr_b16 %2, %4 offset:1024\n\tds_read_b64_tr_b16 %3, %4 offset:1152\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(a[0]), "=&v"(a[1]), "=&v"(a[2]), "=&v"(a[3])
+                     : "v"(at)
+                     : "memory");
+    } else {
+        static_assert(N == 1, "one, two or four operands");
+        asm volatile("ds_read_b64_tr_b16 %0, %2\n\tds_read_b64_tr_b16 %1, %2 offset:128\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(a[0]), "=&v"(a[1])
+                     : "v"(at)
+                     : "memory");
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = mu_join(a[2 * i], a[2 * i + 1]);
 }
 
+#ifndef MU_RING128
+#define MU_RING128 5
+#endif
+#ifndef MU_RING64
+#define MU_RING64 5
+#endif
+template <int TILE>
+__host__ __device__ constexpr int mu_ring() { return TILE == 128 ? MU_RING128 : MU_RING64; }
+
 // acc += operand rows [TILE] x operand columns [TILE] over k steps [k0, k1).  Four waves (2 x 2), wave tile TILE/2 squared.
-// Ring of four stages, one k step each, filled by LDS-DMA three steps ahead; one counted wait and one barrier per step.
+// Ring of NBUF stages, one k step each, filled by LDS-DMA; one counted wait and one barrier per step.  The operands of
+// step i + 1 are read from LDS into a second set of registers under the matrix instructions of step i, and reads and
+// DMAs are dealt out between the matrix instructions: a wave issues in order, and sixteen DMAs of a step take the
+// CU's address unit 256 clk - issued in one go ahead of the products they cost that time in every step.
 // TR: the row operand is X read down its columns (rsrc: tile (0, first n step), nsteps: n steps of a row of tiles).
-template <int TILE, int TERMS, bool TR>
+template <int TILE, int TERMS, bool TR, int NBUF>
 __device__ __forceinline__ void mu_mainloop(const char* rsrc, const char* csrc, int nsteps, int KS, int k0, int k1, char* smem,
                                             mu_acc (&acc)[TILE / 64][TILE / 64]) {
     constexpr int F = TILE / 32, W = TILE / 64;          // tiles per side, of the workgroup and of a wave
     constexpr int NP = TERMS == 3 ? 2 : 1;
     constexpr int SIDE = F * NP, PPW = 2 * SIDE / 4;     // pieces of one side, pieces per wave
-    constexpr int STAGE = 2 * SIDE * MU_FRAG, NBUF = 4;
+    constexpr int STAGE = 2 * SIDE * MU_FRAG;
     const int lane = threadIdx.x & 63;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wid >> 1, wc = wid & 1;
@@ -245,51 +312,71 @@ __device__ __forceinline__ void mu_mainloop(const char* rsrc, const char* csrc, 
         if (tr[i]) src[i] = rsrc + (2L * f + (lane >> 5)) * MU_STEP + part * MU_FRAG + (lane & 31) * 16;
         else src[i] = (side == 0 ? rsrc : csrc) + (long)f * KS * MU_STEP + part * MU_FRAG + lane * 16;
     }
-    auto stage = [&](int buf, int ks) {
-#pragma unroll
-        for (int i = 0; i < PPW; ++i) {
-            const long at = tr[i] ? (long)(ks >> 1) * nsteps * MU_STEP + (ks & 1) * 512 : (long)ks * MU_STEP;
-            __builtin_amdgcn_global_load_lds(MU_GLOBAL_PTR(src[i] + at), MU_LDS_PTR(smem + buf * STAGE + (wid + 4 * i) * MU_FRAG),
-                                             16, 0, 0);
-        }
+    auto stage = [&](int i, int buf, int ks) {
+        const long at = tr[i] ? (long)(ks >> 1) * nsteps * MU_STEP + (ks & 1) * 512 : (long)ks * MU_STEP;
+        __builtin_amdgcn_global_load_lds(MU_GLOBAL_PTR(src[i] + at), MU_LDS_PTR(smem + buf * STAGE + (wid + 4 * i) * MU_FRAG), 16, 0, 0);
     };
-    auto compute = [&](int buf) {
-        const char* sr = smem + buf * STAGE + wr * W * NP * MU_FRAG;
-        const char* sc = smem + buf * STAGE + (SIDE + wc * W * NP) * MU_FRAG;
-        mu_h8 r[W][NP], c[W][NP];
-#pragma unroll
-        for (int i = 0; i < W; ++i)
-#pragma unroll
-            for (int s = 0; s < NP; ++s) {
-                c[i][s] = *reinterpret_cast<const mu_h8*>(sc + (i * NP + s) * MU_FRAG + ln.direct);
-                const char* t = sr + (i * NP + s) * MU_FRAG;
-                if constexpr (TR) r[i][s] = mu_tr(t + ln.tr0, t + ln.tr1);
-                else r[i][s] = *reinterpret_cast<const mu_h8*>(t + ln.direct);
-            }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < W; ++i)
-#pragma unroll
-            for (int j = 0; j < W; ++j) {
-                if constexpr (TERMS == 3) {              // smallest terms first
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[i][1], c[j][0], acc[i][j], 0, 0, 0);
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[i][0], c[j][1], acc[i][j], 0, 0, 0);
-                }
-                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[i][0], c[j][0], acc[i][j], 0, 0, 0);
-            }
-        __builtin_amdgcn_sched_barrier(0);
+    constexpr int OPS = W * NP;                          // operands of a side
+    mu_h8 r[2][OPS], c[2][OPS];
+    const char* my_r = smem + wr * OPS * MU_FRAG + (TR ? ln.tr : ln.direct);
+    const char* my_c = smem + (SIDE + wc * OPS) * MU_FRAG + ln.direct;
+    constexpr int READS = TR ? OPS : 2 * OPS;            // single reads; the transposing ones go as a block
+    auto read = [&](int n, int set, int buf) {
+        if (n < OPS) c[set][n] = *reinterpret_cast<const mu_h8*>(my_c + buf * STAGE + n * MU_FRAG);
+        else r[set][n - OPS] = *reinterpret_cast<const mu_h8*>(my_r + buf * STAGE + (n - OPS) * MU_FRAG);
+    };
+    constexpr int MF = (TERMS == 3 ? 3 : 1) * W * W;     // matrix instructions of a step
+    auto multiply = [&](int n, int set) {
+        const int t = n / (W * W), i = n / W % W, j = n % W;      // smallest terms first; a term of all blocks, then the next
+        const int pr = TERMS == 3 && t == 0 ? 1 : 0, pc = TERMS == 3 && t == 1 ? 1 : 0;
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[set][i * NP + pr], c[set][j * NP + pc], acc[i][j], 0, 0, 0);
     };
     const int nk = k1 - k0;
     if (nk <= 0) return;
     // past the end the last step is fetched again, into a buffer nobody reads any more: every wave always has the same
     // number of operations in flight, and one counted wait fits every iteration
 #pragma unroll
-    for (int s = 0; s < NBUF - 1; ++s) stage(s, k0 + min(s, nk - 1));
-    for (int it = 0; it < nk; ++it) {
-        // own pieces of step `it` have landed, own reads of step it - 1 are done; after the barrier everybody's
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NBUF - 2) * PPW) : "memory");
-        stage((it + NBUF - 1) % NBUF, k0 + min(it + NBUF - 1, nk - 1));
-        compute(it % NBUF);
+    for (int s = 0; s < NBUF - 1; ++s)
+#pragma unroll
+        for (int i = 0; i < PPW; ++i) stage(i, s, k0 + min(s, nk - 1));
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NBUF - 2) * PPW) : "memory");
+#pragma unroll
+    for (int n = 0; n < READS; ++n) read(n, 0, 0);
+    if constexpr (TR) mu_tr_block(my_r, r[0]);
+    int b_read = 1, b_fill = NBUF - 1;
+    // step `it`: its operands are in (or on their way to) register set `set`
+    auto step = [&](int set, int it) {
+        // own pieces of step it + 1 have landed, own reads of step it are done: after the barrier everybody's, and the buffer
+        // of step it - 1 (read before the previous barrier) is free
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NBUF - 3) * PPW) : "memory");
+        const int fill = k0 + min(it + NBUF - 1, nk - 1);
+        constexpr int HALF = MF * 2 / 3 > 0 ? MF * 2 / 3 : 1;      // reads go first: they have to be back by the next step
+#pragma unroll
+        for (int n = 0; n < MF; ++n) {
+            multiply(n, set);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < READS; ++k)
+                if (k * HALF / READS == n) read(k, set ^ 1, b_read);
+            if constexpr (TR) {
+                if (n == MF / 2) mu_tr_block(my_r + b_read * STAGE, r[set ^ 1]);
+            }
+#pragma unroll
+            for (int k = 0; k < PPW; ++k)
+                if (((k + 1) * MF - 1) / PPW == n) stage(k, b_fill, fill);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        b_fill = b_fill + 1 == NBUF ? 0 : b_fill + 1;
+        b_read = b_read + 1 == NBUF ? 0 : b_read + 1;
+    };
+    int it = 0;
+    for (; it + 1 < nk; it += 2) {
+        step(0, it);
+        step(1, it + 1);
+    }
+    if (it < nk) {
+#pragma unroll
+        for (int n = 0; n < MF; ++n) multiply(n, 0);
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the epilogue reuses the stages
 }
@@ -314,13 +401,23 @@ __device__ __forceinline__ void mu_put(char* at, const float (&v)[4]) {
     *reinterpret_cast<mu_h4*>(at) = hi;
     if constexpr (NP == 2) *reinterpret_cast<mu_h4*>(at + MU_FRAG) = lo;
 }
+// the same place read: a block's worth at once (16 values per lane), before anything is stored - a load behind a store that
+// might alias it waits for its own round trip, sixteen times in a tile
+struct MuOld {
+    mu_h4 hi[4], lo[4];
+};
 template <int NP>
-__device__ __forceinline__ void mu_get(const char* at, float (&v)[4]) {
-    const mu_h4 hi = *reinterpret_cast<const mu_h4*>(at);
-    mu_h4 lo = {0, 0, 0, 0};
-    if constexpr (NP == 2) lo = *reinterpret_cast<const mu_h4*>(at + MU_FRAG);
+__device__ __forceinline__ void mu_load_block(MuOld& o, const char* fm, int rt, int KS, int kr, int lane) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = (float)hi[k] + (float)lo[k];
+    for (int q = 0; q < 4; ++q) {
+        const char* at = fm + mu_block_at(rt, KS, kr, q, lane);
+        o.hi[q] = *reinterpret_cast<const mu_h4*>(at);
+        if constexpr (NP == 2) o.lo[q] = *reinterpret_cast<const mu_h4*>(at + MU_FRAG);
+    }
+}
+template <int NP>
+__device__ __forceinline__ float mu_old(const MuOld& o, int q, int k) {
+    return NP == 2 ? (float)o.hi[q][k] + (float)o.lo[q][k] : (float)o.hi[q][k];
 }
 
 // LDS written by some lanes of the wave, read by others: the hardware keeps a wave's LDS operations in order, the
@@ -330,53 +427,61 @@ __device__ __forceinline__ void mu_wave_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// a tile of a symmetric matrix (tile row ti of k, tile column tj of rows), and its mirror image: transposed per 32 x 32
-// block through 4 KiB of LDS that belong to the wave
+// One 32 x 32 block of a symmetric matrix: rb counts along k of the direct image, cb along its rows.  `mirror`: also the block
+// on the other side of the diagonal, transposed through 4 KiB of LDS that belong to the wave.
+template <int NP, bool POLY>
+__device__ __forceinline__ void mu_emit_block(const mu_acc& acc, char* dst, const MuOld& old, int KS, int rb, int cb, bool mirror,
+                                              const MuScale& sc, char* mine) {
+    const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        float v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = acc[4 * q + k] * sc.f_acc + (POLY ? mu_old<NP>(old, q, k) * sc.f_add : 0.0f);
+        mu_put<NP>(dst + mu_block_at(cb, KS, rb * 32, q, lane), v);
+        if (mirror) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int row = 8 * q + 4 * h + k;
+                _Float16 hi, lo;
+                mu_parts(v[k], hi, lo);
+                char* t = mine + (col >> 4) * 1024 + mu_at(row, (col >> 3) & 1) + (col & 7) * 2;
+                *reinterpret_cast<_Float16*>(t) = hi;
+                if constexpr (NP == 2) *reinterpret_cast<_Float16*>(t + 2048) = lo;
+            }
+        }
+    }
+    if (mirror) {
+        mu_wave_fence();
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+                const mu_h8 v = *reinterpret_cast<const mu_h8*>(mine + p * 2048 + s * 1024 + lane * 16);
+                *reinterpret_cast<mu_h8*>(dst + ((long)rb * KS + cb * 2 + s) * MU_STEP + p * MU_FRAG + lane * 16) = v;
+            }
+        mu_wave_fence();
+    }
+}
+// a tile of it (tile row ti of k, tile column tj of rows)
 template <int TILE, int TERMS, bool POLY>
 __device__ __forceinline__ void mu_emit_sym(mu_acc (&acc)[TILE / 64][TILE / 64], char* dst, const char* add, int KS, int ti, int tj,
                                             const MuScale& sc, char* smem) {
-    constexpr int W = TILE / 64, NP = TERMS == 3 ? 2 : 1, F = TILE / 32;
-    const int lane = threadIdx.x & 63;
+    constexpr int W = TILE / 64, F = TILE / 32, NP = TERMS == 3 ? 2 : 1;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wr = wid >> 1, wc = wid & 1, col = lane & 31, h = lane >> 5;
-    char* mine = smem + wid * 4096;
+    const int rb0 = ti * F + (wid >> 1) * W, cb0 = tj * F + (wid & 1) * W;
+    MuOld old[W][W];
+    if constexpr (POLY) {
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+#pragma unroll
+            for (int j = 0; j < W; ++j) mu_load_block<NP>(old[i][j], add, cb0 + j, KS, (rb0 + i) * 32, threadIdx.x & 63);
+    }
 #pragma unroll
     for (int i = 0; i < W; ++i)
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
-            const int rb = ti * F + wr * W + i, cb = tj * F + wc * W + j;       // 32-blocks: k of the direct image, rows
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                float v[4], old[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                const long at = mu_block_at(cb, KS, rb * 32, q, lane);
-                if constexpr (POLY) mu_get<NP>(add + at, old);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] = acc[i][j][4 * q + k] * sc.f_acc + (POLY ? old[k] * sc.f_add : 0.0f);
-                mu_put<NP>(dst + at, v);
-                if (ti != tj) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int row = 8 * q + 4 * h + k;
-                        _Float16 hi, lo;
-                        mu_parts(v[k], hi, lo);
-                        char* t = mine + (col >> 4) * 1024 + mu_at(row, (col >> 3) & 1) + (col & 7) * 2;
-                        *reinterpret_cast<_Float16*>(t) = hi;
-                        if constexpr (NP == 2) *reinterpret_cast<_Float16*>(t + 2048) = lo;
-                    }
-                }
-            }
-            if (ti != tj) {
-                mu_wave_fence();
-#pragma unroll
-                for (int s = 0; s < 2; ++s)
-#pragma unroll
-                    for (int p = 0; p < NP; ++p) {
-                        const mu_h8 v = *reinterpret_cast<const mu_h8*>(mine + p * 2048 + s * 1024 + lane * 16);
-                        *reinterpret_cast<mu_h8*>(dst + ((long)rb * KS + cb * 2 + s) * MU_STEP + p * MU_FRAG + lane * 16) = v;
-                    }
-                mu_wave_fence();
-            }
-        }
+        for (int j = 0; j < W; ++j)
+            mu_emit_block<NP, POLY>(acc[i][j], dst, old[i][j], KS, rb0 + i, cb0 + j, ti != tj, sc, smem + wid * 4096);
 }
 
 // tile t of the upper triangle, column by column: (i <= j)
@@ -385,6 +490,19 @@ __device__ __forceinline__ void mu_pair(int t, int& i, int& j) {
     while ((j + 1) * (j + 2) / 2 <= t) ++j;
     while (j * (j + 1) / 2 > t) --j;
     i = t - j * (j + 1) / 2;
+}
+// the same tiles in bands of eight columns, rows of a band one after the other: 64 neighbours share 8 + 8 operand panels
+__device__ __forceinline__ void mu_pair_banded(int t, int T, int& i, int& j) {
+    mu_pair(t, i, j);
+    const int j0 = j & ~7, w = min(8, T - j0), r = t - j0 * (j0 + 1) / 2, rect = j0 * w;
+    if (r < rect) {
+        i = r / w;
+        j = j0 + r - i * w;
+    } else {
+        mu_pair(r - rect, i, j);
+        i += j0;
+        j += j0;
+    }
 }
 
 // workgroups of one XCD (every eighth) take consecutive tiles, which share operand panels through its L2
@@ -406,7 +524,7 @@ __global__ __launch_bounds__(256) void mu_sym_kernel(MuTab tab, int total, char*
     const int local = tl - tab.start[e], mat = local / (ntri * splits), rest = local - mat * ntri * splits;
     const int s = rest / ntri, t = rest - s * ntri;
     int ti, tj;
-    mu_pair(t, ti, tj);
+    mu_pair_banded(t, T, ti, tj);
     char* base = ws + ge.off + mat * mu_matrix_bytes<TILE>(ge);
     const long xs = 4L * ge.mp * ge.np, as = 4L * ge.mp * ge.mp;
     char* A = base + 2 * xs;
@@ -421,7 +539,7 @@ __global__ __launch_bounds__(256) void mu_sym_kernel(MuTab tab, int total, char*
 #pragma unroll
             for (int k = 0; k < 16; ++k) acc[i][j][k] = 0.0f;
     const long rows = (long)(TILE / 32) * KS * MU_STEP;
-    mu_mainloop<TILE, TERMS, false>(src + ti * rows, src + tj * rows, 0, KS, MODE == MU_GRAM ? k0 : 0, k1, smem, acc);
+    mu_mainloop<TILE, TERMS, false, mu_ring<TILE>()>(src + ti * rows, src + tj * rows, 0, KS, MODE == MU_GRAM ? k0 : 0, k1, smem, acc);
     if (MODE == MU_GRAM && splits > 1) {
         // this split's share, as the registers lie (the reducing kernel has the same lanes): 256 bytes per store
         float* part = reinterpret_cast<float*>(A + 2 * as) + ((long)s * ntri + t) * TILE * TILE;
@@ -440,43 +558,41 @@ __global__ __launch_bounds__(256) void mu_sym_kernel(MuTab tab, int total, char*
     mu_emit_sym<TILE, TERMS, MODE == MU_POLY>(acc, MODE == MU_POLY ? A + as : A, A, ge.mp >> 4, ti, tj, sc, smem);
 }
 
-// the sum of the splits in fixed order, then what the product kernel does when there is one
+// The sum of the splits in fixed order, then what the product kernel does when there is one.  A wave per 32 x 32 block (the
+// blocks of a tile lie one after the other in a share): 16 of them per tile, for there are few tiles where there are splits.
 template <int TILE, int TERMS>
 __global__ __launch_bounds__(256) void mu_reduce_kernel(MuTab tab, char* __restrict__ ws, MuScale sc) {
     __shared__ __attribute__((aligned(1024))) char smem[4 * 4096];
-    const int e = mu_entry(tab, blockIdx.x);
+    constexpr int W = TILE / 64, WGS = W * W;              // workgroups per tile, four blocks each
+    const int e = mu_entry(tab, blockIdx.x / WGS);
     const MuGeo& ge = tab.e[e];
     if (ge.splits == 1) return;
     const int T = ge.mp / TILE, ntri = T * (T + 1) / 2;
-    const int local = blockIdx.x - tab.start[e], mat = local / ntri, t = local - mat * ntri;
+    const int local = blockIdx.x / WGS - tab.start[e], mat = local / ntri, t = local - mat * ntri;
     int ti, tj;
-    mu_pair(t, ti, tj);
+    mu_pair_banded(t, T, ti, tj);
     char* base = ws + ge.off + mat * mu_matrix_bytes<TILE>(ge);
     const long xs = 4L * ge.mp * ge.np, as = 4L * ge.mp * ge.mp;
     char* A = base + 2 * xs;
-    const float* part = reinterpret_cast<const float*>(A + 2 * as) + (long)t * TILE * TILE;
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-    mu_acc acc[TILE / 64][TILE / 64];
+    const int block = (blockIdx.x % WGS) * 4 + wid;        // (wave of the product kernel, i, j)
+    const mu_f4* part = reinterpret_cast<const mu_f4*>(A + 2 * as) + ((long)t * 4 * WGS + block) * 256 + lane;
+    mu_acc acc;
 #pragma unroll
-    for (int i = 0; i < TILE / 64; ++i)
-#pragma unroll
-        for (int j = 0; j < TILE / 64; ++j)
-#pragma unroll
-            for (int k = 0; k < 16; ++k) acc[i][j][k] = 0.0f;
+    for (int k = 0; k < 16; ++k) acc[k] = 0.0f;
+#pragma unroll 4
     for (int s = 0; s < ge.splits; ++s) {
-        const mu_f4* p = reinterpret_cast<const mu_f4*>(part + (long)s * ntri * TILE * TILE);
+        const mu_f4* p = part + (long)s * ntri * (TILE * TILE / 4);
 #pragma unroll
-        for (int i = 0; i < TILE / 64; ++i)
+        for (int q = 0; q < 4; ++q) {
+            const mu_f4 v = p[q * 64];
 #pragma unroll
-            for (int j = 0; j < TILE / 64; ++j)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const mu_f4 v = p[((wid * (TILE / 64) + i) * (TILE / 64) + j) * 256 + q * 64 + lane];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) acc[i][j][4 * q + k] += v[k];
-                }
+            for (int k = 0; k < 4; ++k) acc[4 * q + k] += v[k];
+        }
     }
-    mu_emit_sym<TILE, TERMS, false>(acc, A, nullptr, ge.mp >> 4, ti, tj, sc, smem);
+    const int w = block / WGS, ij = block % WGS;
+    const int rb = ti * (TILE / 32) + (w >> 1) * W + ij / W, cb = tj * (TILE / 32) + (w & 1) * W + ij % W;
+    mu_emit_block<TERMS == 3 ? 2 : 1, false>(acc, A, MuOld(), ge.mp >> 4, rb, cb, ti != tj, sc, smem + wid * 4096);
 }
 
 // where a finished result goes: out = v, or the parameter step p <- decay p - lr_scale v (one rounding to T)
@@ -497,7 +613,9 @@ __global__ __launch_bounds__(256) void mu_step_kernel(MuTab tab, int total, MuPt
     const MuGeo& ge = tab.e[e];
     const int TM = ge.mp / TILE, TN = ge.np / TILE;
     const int local = tl - tab.start[e], mat = local / (TM * TN), rest = local - mat * TM * TN;
-    const int tn = rest / TM, tm = rest - tn * TM;
+    // bands of eight tile columns, rows of a band one after the other: 64 neighbours share 8 + 8 operand panels
+    const int n0 = rest / (8 * TM) * 8, w = min(8, TN - n0), inband = rest - n0 * TM;
+    const int tm = inband / w, tn = n0 + inband - tm * w;
     char* base = ws + ge.off + mat * mu_matrix_bytes<TILE>(ge);
     const long xs = 4L * ge.mp * ge.np, as = 4L * ge.mp * ge.mp;
     const char* X = base + ping * xs;
@@ -512,36 +630,69 @@ __global__ __launch_bounds__(256) void mu_step_kernel(MuTab tab, int total, MuPt
         for (int j = 0; j < W; ++j)
 #pragma unroll
             for (int k = 0; k < 16; ++k) acc[i][j][k] = 0.0f;
-    mu_mainloop<TILE, TERMS, true>(X + (long)tn * (TILE / 16) * MU_STEP, B + (long)tm * F * KS * MU_STEP, NS, KS, 0, KS, smem, acc);
+    mu_mainloop<TILE, TERMS, true, mu_ring<TILE>()>(X + (long)tn * (TILE / 16) * MU_STEP, B + (long)tm * F * KS * MU_STEP, NS, KS, 0, KS, smem, acc);
     const int lane = threadIdx.x & 63;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wid >> 1, wc = wid & 1, h = lane >> 5;
     const long len = (long)ge.m * ge.n;
     T* out = LAST ? static_cast<T*>(ptrs.p[e]) + mat * len : nullptr;
+    MuOld old[W][W];
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+            mu_load_block<2>(old[i][j], X, tm * F + wc * W + j, NS, (tn * F + wr * W + i) * 32, lane);
 #pragma unroll
     for (int i = 0; i < W; ++i)
 #pragma unroll
         for (int j = 0; j < W; ++j) {
             const int nb = tn * F + wr * W + i, mb = tm * F + wc * W + j;
+            float v[16];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const long at = mu_block_at(mb, NS, nb * 32, q, lane);
-                float v[4], x[4];
-                mu_get<2>(X + at, x);
+            for (int q = 0; q < 4; ++q)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] = acc[i][j][4 * q + k] * sc.f_acc + x[k] * sc.f_add;
-                if constexpr (!LAST) {
-                    mu_put<2>(Y + at, v);
-                } else {
-                    const int m = mb * 32 + (lane & 31), n = nb * 32 + 8 * q + 4 * h;
-                    if (m < ge.m) {
+                for (int k = 0; k < 4; ++k) v[4 * q + k] = acc[i][j][4 * q + k] * sc.f_acc + mu_old<2>(old[i][j], q, k) * sc.f_add;
+            if constexpr (!LAST) {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            if (n + k < ge.n)
-                                mu_finish(out, ge.trans ? (long)(n + k) * ge.m + m : (long)m * ge.n + n + k, v[k], decay,
-                                          ptrs.lr_scale[e], is_step != 0);
-                    }
+                for (int q = 0; q < 4; ++q) {
+                    const float four[4] = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+                    mu_put<2>(Y + mu_block_at(mb, NS, nb * 32, q, lane), four);
                 }
+            } else {
+                // lanes along the caller's contiguous dimension: m as it is, n through 32 x 33 floats that belong to the wave
+                long at[16];
+                bool ok[16];
+                if (ge.trans) {
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const int m = mb * 32 + (lane & 31), n = nb * 32 + 8 * (k >> 2) + 4 * h + (k & 3);
+                        at[k] = (long)n * ge.m + m;
+                        ok[k] = m < ge.m && n < ge.n;
+                    }
+                } else {
+                    float* mine = reinterpret_cast<float*>(smem) + wid * 32 * 33;
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) mine[(lane & 31) * 33 + 8 * (k >> 2) + 4 * h + (k & 3)] = v[k];
+                    mu_wave_fence();
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        v[k] = mine[(2 * k + h) * 33 + (lane & 31)];
+                        const int m = mb * 32 + 2 * k + h, n = nb * 32 + (lane & 31);
+                        at[k] = (long)m * ge.n + n;
+                        ok[k] = m < ge.m && n < ge.n;
+                    }
+                    mu_wave_fence();
+                }
+                if (is_step) {
+                    T p[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) p[k] = ok[k] ? out[at[k]] : (T)0.0f;
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) v[k] = decay * (float)p[k] - ptrs.lr_scale[e] * v[k];
+                }
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                    if (ok[k]) out[at[k]] = (T)v[k];
             }
         }
 }
@@ -669,11 +820,12 @@ __global__ __launch_bounds__(MU_SMALL_NT) void mu_small_kernel(MuTab tab, MuPtrs
         float v4[4][4];
         if (mine) {
             product(A + rb * KS * MU_STEP, A + cb * KS * MU_STEP, KS, acc);
+            MuOld old;
+            mu_load_block<NP>(old, A, cb, KS, rb * 32, lane);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                mu_get<NP>(A + mu_block_at(cb, KS, rb * 32, q, lane), v4[q]);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) v4[q][k] = acc[4 * q + k] * st.poly[it].f_acc + v4[q][k] * st.poly[it].f_add;
+                for (int k = 0; k < 4; ++k) v4[q][k] = acc[4 * q + k] * st.poly[it].f_acc + mu_old<NP>(old, q, k) * st.poly[it].f_add;
             }
         }
         __syncthreads();
@@ -698,17 +850,15 @@ __global__ __launch_bounds__(MU_SMALL_NT) void mu_small_kernel(MuTab tab, MuPtrs
                         // the two n steps of a block are 2 KiB apart here, not 512 bytes
                         const char* t = X + ((ks >> 1) * NS + nb * 2) * MU_STEP + s * MU_FRAG + (ks & 1) * 512 +
                                         ((lane >> 4) & 1) * (MU_STEP - 512);
-                        r[s] = mu_tr(t + ln.tr0, t + ln.tr1);
+                        r[s] = mu_tr(t + ln.tr);
                     }
                     mfma(r, c, y[b]);
                 }
+                MuOld old;
+                mu_load_block<2>(old, X, mb, NS, nb * 32, lane);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    float x[4];
-                    mu_get<2>(X + mu_block_at(mb, NS, nb * 32, q, lane), x);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) y[b][4 * q + k] = y[b][4 * q + k] * st.step[it].f_acc + x[k] * st.step[it].f_add;
-                }
+                for (int k = 0; k < 16; ++k)
+                    y[b][k] = y[b][k] * st.step[it].f_acc + mu_old<2>(old, k >> 2, k & 3) * st.step[it].f_add;
             }
         }
         __syncthreads();
@@ -805,7 +955,13 @@ static bool mu_small(const MuJob& j) {
     return m <= 128 && n <= MU_SMALL_ENTRIES && m * n + m * m <= MU_SMALL_ENTRIES;
 }
 
-constexpr int MU_TARGET_WGS = 512;               // two workgroups per CU: what the splits of X X^T aim at
+#ifndef MU_TW
+#define MU_TW 512
+#endif
+#ifndef MU_TMIN
+#define MU_TMIN 16
+#endif
+constexpr int MU_TARGET_WGS = MU_TW;               // two workgroups per CU: what the splits of X X^T aim at
 constexpr long MU_PASS_BYTES = 1L << 30;         // workspace beyond which a batch is run in several passes
 constexpr long MU_MAX_SIDE = 65536, MU_MAX_LONG = 1L << 24, MU_MAX_ENTRIES = 1L << 36;
 
@@ -843,7 +999,7 @@ static void mu_plan(const MuJob* jobs, int n, MuPlan& pl) {
         work += jobs[i].count * mu_tri(g.mp / tile) * (g.np / 16);
     }
     // k steps per workgroup of X X^T so that all of them together fill the chip, no fewer than 16
-    const long target = std::max(16L, (work + MU_TARGET_WGS - 1) / MU_TARGET_WGS);
+    const long target = std::max((long)MU_TMIN, (work + MU_TARGET_WGS - 1) / MU_TARGET_WGS);
     pl.norm_blocks = 0;
     for (int i = 0; i < n; ++i) {
         MuGeo& g = pl.geo[i];
@@ -949,8 +1105,16 @@ static int mu_run_tiled(const MuJob* jobs, const MuPlan& pl, const MuRun& r, cha
     hipLaunchKernelGGL((mu_split_kernel<T>), dim3(n_split), dim3(256), 0, r.stream, tsplit, norm, pt, r.mm, r.co.eps, r.x0_scale,
                        (const double*)partial, ws, TILE == 128 ? 1 : 0);
     MV_LAUNCH_CHECK("mu_split_kernel");
-    constexpr size_t lds = (size_t)4 * 2 * (TILE / 32) * (TERMS == 3 ? 2 : 1) * MU_FRAG;
-    static_assert(lds <= 64 * 1024 && lds >= 4 * 4096, "the ring fits the default LDS limit and holds the mirror's blocks");
+    constexpr size_t lds = (size_t)mu_ring<TILE>() * 2 * (TILE / 32) * (TERMS == 3 ? 2 : 1) * MU_FRAG;
+    static_assert(lds <= 160 * 1024 && lds >= 4 * 4224, "the ring fits LDS and holds the epilogues blocks");
+    const void* kernels[4] = {reinterpret_cast<const void*>(mu_sym_kernel<TILE, TERMS, MU_GRAM>),
+                              reinterpret_cast<const void*>(mu_sym_kernel<TILE, TERMS, MU_POLY>),
+                              reinterpret_cast<const void*>(mu_step_kernel<T, TILE, TERMS, false>),
+                              reinterpret_cast<const void*>(mu_step_kernel<T, TILE, TERMS, true>)};
+    for (const void* k : kernels) {
+        const hipError_t e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        MV_REQUIRE(e == hipSuccess, (int)e, "mu_sym_kernel: cannot raise the LDS limit: %s", hipGetErrorString(e));
+    }
     auto grid = [](int n) { return dim3((unsigned)((n + 7) / 8 * 8)); };
     for (int it = 0; it < r.st.steps; ++it) {
         const int ping = it & 1;
@@ -958,7 +1122,7 @@ static int mu_run_tiled(const MuJob* jobs, const MuPlan& pl, const MuRun& r, cha
                            r.st.gram[it]);
         MV_LAUNCH_CHECK("mu_sym_kernel");
         if (split) {
-            hipLaunchKernelGGL((mu_reduce_kernel<TILE, TERMS>), dim3(n_poly), dim3(256), 0, r.stream, tpoly, ws, r.st.gram[it]);
+            hipLaunchKernelGGL((mu_reduce_kernel<TILE, TERMS>), dim3(n_poly * (TILE / 64) * (TILE / 64)), dim3(256), 0, r.stream, tpoly, ws, r.st.gram[it]);
             MV_LAUNCH_CHECK("mu_reduce_kernel");
         }
         hipLaunchKernelGGL((mu_sym_kernel<TILE, TERMS, MU_POLY>), grid(n_poly), dim3(256), lds, r.stream, tpoly, n_poly, ws, ping,
