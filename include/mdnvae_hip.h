@@ -735,7 +735,7 @@ int mdnvae_muon_step(void* const* params, const void* const* grads, float* const
  *     grad = dloss / dlogits [T][E] in the logits' type, zeros in rows that are not valid; NULL: not wanted
  * A logit of -inf masks that expert out of that row (p = 0, never counted), a row of nothing else is not valid.  A NaN or
  * +inf in a valid row gives NaN there (NaN counts as the largest number).  n = 0: zeros.  Logits of rows that are not
- * valid are never looked at.  Sums in fixed order. */
+ * valid are never looked at.  n_valid may be NULL.  Sums in fixed order. */
 size_t mdnvae_gate_balance_workspace_bytes(long T, int E);
 int mdnvae_gate_balance(const void* logits, const unsigned char* valid, long T, int E, int top_k, int dtype, void* workspace,
                         size_t workspace_bytes, float* loss, int* counts, float* mean_probs, int* n_valid, void* grad,

@@ -10,11 +10,13 @@
 // row of nothing else is not valid; NaN counts as larger than every number.
 //
 // Two sweeps over the logits, since every gradient depends on the counts of all rows: statistics, then gradient.  A row
-// belongs to a group of L lanes, eight (sixteen above 512 experts) values each; experts stay with their lane, so sums of
+// belongs to a group of L lanes, eight (sixteen above 128 experts) values each; experts stay with their lane, so sums of
 // p and counts are kept in registers over all rows of a wave and leave once per workgroup.  Selection: every lane sorts its
-// keys once (a network of 19 exchanges), then k rounds of "largest head of the group, its lane moves on" find the
+// keys once (a network of 19 or 63 exchanges), then k rounds of "largest head of the group, its lane moves on" find the
 // k-th largest key; whoever is above it is taken, and of those equal to it as many of the lowest index as are
-// missing (ballots; only where the group saw a tie).
+// missing (ballots; only where the group saw a tie).  Sixteen lanes of sixteen values rather than thirty-two of eight for 256
+// experts: four rows per wave share each round, and all its exchanges stay within a DPP row (290 -> 95 us for 262144 rows,
+// 2.8 TB/s: bound by its instructions, about 620 per four rows).
 #include <algorithm>
 #include "common.h"
 #include "../../include/mdnvae_hip.h"
@@ -38,7 +40,7 @@ __device__ __forceinline__ unsigned gt_key(float z) {
 // reductions over groups of L consecutive lanes; every lane gets the result
 template <int CTRL>
 __device__ __forceinline__ unsigned gt_dpp(unsigned v) {
-    return (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false);
+    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
 }
 template <int L, typename F>
 __device__ __forceinline__ unsigned gt_reduce(unsigned v, F f) {
@@ -67,6 +69,17 @@ __device__ __forceinline__ float gt_sum(float v) {
     }));
 }
 
+// exp(x), x <= 0 (or NaN, -inf): 2^t by the hardware with t = x log2 e rounded, and what the rounding left out as a first-order
+// factor - a couple of 2^-24 for all x, at a third of the instructions of expf
+__device__ __forceinline__ float gt_exp(float x) {
+    const float log2e = 1.44269504f, tail = 1.92596299e-8f, ln2 = 0.693147181f;
+    const float y = fmaxf(x, -150.0f);                      // zero either way; keeps -inf out of the remainder (NaN: below)
+    const float t = y * log2e;
+    const float rest = fmaf(y, log2e, -t) + y * tail;
+    const float p = __builtin_amdgcn_exp2f(t);
+    return x != x ? x : fmaf(p, rest * ln2, p);
+}
+
 template <typename T, int L, int NV, int VEC>
 __device__ __forceinline__ void gt_load(const T* row, int E, int l, bool in, float (&z)[NV]) {
     typedef T vec __attribute__((ext_vector_type(4)));
@@ -85,7 +98,22 @@ __device__ __forceinline__ void gt_load(const T* row, int E, int l, bool in, flo
     }
 }
 
-// softmax of a row in place; false (and zeros) where the row has no expert left
+// softmax of a row in place, m its largest logit; false (and zeros) where the row has no expert left
+template <int L, int NV>
+__device__ __forceinline__ bool gt_softmax_at(float (&z)[NV], float m) {
+    float s = 0.0f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        z[v] = gt_exp(z[v] - m);
+        s += z[v];
+    }
+    s = gt_sum<L>(s);
+    const float inv = 1.0f / s;
+    const bool any = m != -INFINITY;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) z[v] = any ? z[v] * inv : 0.0f;
+    return any;
+}
 template <int L, int NV>
 __device__ __forceinline__ bool gt_softmax(float (&z)[NV]) {
     float m = z[0];
@@ -96,18 +124,7 @@ __device__ __forceinline__ bool gt_softmax(float (&z)[NV]) {
         nan = nan || z[v] != z[v];
     }
     if (nan) m = INFINITY;                                  // a NaN shows in every probability of the row
-    m = gt_fmax<L>(m);
-    float s = 0.0f;
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-        z[v] = m == -INFINITY ? 0.0f : expf(z[v] - m);
-        s += z[v];
-    }
-    s = gt_sum<L>(s);
-    const float inv = 1.0f / s;
-#pragma unroll
-    for (int v = 0; v < NV; ++v) z[v] = m == -INFINITY ? 0.0f : z[v] * inv;
-    return m != -INFINITY;
+    return gt_softmax_at<L, NV>(z, gt_fmax<L>(m));
 }
 
 __device__ __forceinline__ void gt_exchange(unsigned& a, unsigned& b) {    // a >= b afterwards
@@ -129,21 +146,46 @@ __device__ __forceinline__ void gt_sort(unsigned (&s)[N]) {
                     if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) gt_exchange(s[i + j], s[i + j + k]);
 }
 
-// which slots of the row are among its top_k: bit v of the result
+// top_k rounds on sorted lists of which the first D entries can matter; the lists' next heads
+template <int L, int NV, int D>
+__device__ __forceinline__ unsigned gt_rounds(const unsigned (&sorted)[NV], int top_k, int lane, unsigned& first, unsigned& t, int& need) {
+    const int base = lane & ~(L - 1), l = lane & (L - 1);
+    unsigned s[D];
+#pragma unroll
+    for (int v = 0; v < D; ++v) s[v] = sorted[v];
+    for (int r = 0; r < top_k; ++r) {
+        const unsigned m = gt_max<L>(s[0]);
+        if (r == 0) first = m;
+        need = m == t ? need + 1 : 1;
+        t = m;
+        const unsigned long long heads = __ballot(s[0] == m) >> base;     // bit 0: the group's first lane
+        bool own;
+        if constexpr (L == 64) own = l == __ffsll((long long)heads) - 1;
+        else own = l == __ffs((int)(unsigned)(heads & ((1ull << (L & 63)) - 1ull))) - 1;
+        const unsigned move = own ? ~0u : 0u;               // as a mask: "own ? s[v + 1] : s[v]" becomes an indexed register read
+#pragma unroll
+        for (int v = 0; v + 1 < D; ++v) s[v] = (s[v + 1] & move) | (s[v] & ~move);
+        s[D - 1] &= ~move;
+    }
+    return s[0];
+}
+
+// Which slots of the row are among its top_k: those with key >= the result (keys that lose a tie are cleared).  largest: the
+// row's largest logit (+inf where it holds a NaN).
 template <int L, int NV, int VEC>
-__device__ __forceinline__ unsigned gt_select(const float (&z)[NV], int top_k) {
-    unsigned key[NV], s[NV];
+__device__ __forceinline__ unsigned gt_select(const float (&z)[NV], int top_k, unsigned (&key)[NV], float& largest) {
+    unsigned s[NV];
 #pragma unroll
     for (int v = 0; v < NV; ++v) s[v] = key[v] = gt_key(z[v]);
     const int lane = threadIdx.x & 63, base = lane & ~(L - 1);
-    const unsigned long long group = (L == 64 ? ~0ull : ((1ull << L) - 1ull)) << base;
-    unsigned t = 0;
+    const unsigned long long group = (L == 64 ? ~0ull : ((1ull << (L & 63)) - 1ull)) << base;
+    unsigned t = 0, first = 0;
     int need = 0;
     bool tie;
     if (top_k == 1) {
 #pragma unroll
         for (int v = 1; v < NV; ++v) s[0] = s[0] > s[v] ? s[0] : s[v];
-        t = gt_max<L>(s[0]);
+        first = t = gt_max<L>(s[0]);
         need = 1;
         int same = 0;
 #pragma unroll
@@ -151,22 +193,13 @@ __device__ __forceinline__ unsigned gt_select(const float (&z)[NV], int top_k) {
         tie = same > 1 || __popcll(__ballot(same > 0) & group) > 1;
     } else {
         gt_sort<NV>(s);
-        for (int r = 0; r < top_k; ++r) {
-            const unsigned m = gt_max<L>(s[0]);
-            need = m == t ? need + 1 : 1;
-            t = m;
-            const unsigned long long heads = __ballot(s[0] == m) & group;
-            const bool own = lane == __ffsll((long long)heads) - 1;
-#pragma unroll
-            for (int v = 0; v + 1 < NV; ++v) s[v] = own ? s[v + 1] : s[v];
-            s[NV - 1] = own ? 0u : s[NV - 1];
-        }
-        tie = s[0] == t;
+        // a lane gives at most top_k entries, and the one after them is looked at for ties
+        const unsigned next = NV > 9 && top_k < 9 ? gt_rounds<L, NV, NV < 9 ? NV : 9>(s, top_k, lane, first, t, need)
+                                                  : gt_rounds<L, NV, NV>(s, top_k, lane, first, t, need);
+        tie = next == t;
     }
-    unsigned sel = 0;
+    largest = first == 0xffffffffu ? INFINITY : __uint_as_float((first >> 31) ? first & 0x7fffffffu : ~first);
     const unsigned floor_key = t > GT_NEG_INF ? t : GT_NEG_INF + 1;       // nothing at or below -inf is ever taken
-#pragma unroll
-    for (int v = 0; v < NV; ++v) sel |= key[v] >= floor_key ? 1u << v : 0u;
     if (__ballot(tie && t > GT_NEG_INF)) {
         // among the keys equal to t the lowest `need` indices stay: experts are ordered by (chunk, lane, place in the chunk)
         const unsigned long long below = group & ((1ull << lane) - 1ull);
@@ -184,13 +217,13 @@ __device__ __forceinline__ unsigned gt_select(const float (&z)[NV], int top_k) {
 #pragma unroll
             for (int i = 0; i < VEC; ++i)
                 if (key[j * VEC + i] == t) {
-                    if (at >= need) sel &= ~(1u << (j * VEC + i));
+                    if (at >= need) key[j * VEC + i] = 0u;
                     ++at;
                 }
             before += all;
         }
     }
-    return sel;
+    return floor_key;
 }
 
 struct GateArgs {
@@ -221,12 +254,14 @@ __device__ __forceinline__ void gt_stats(const GateArgs& a, long wave_first, lon
     if (wave_first < a.T) fetch(wave_first, z);
     for (long r0 = wave_first; r0 < a.T; r0 += stride) {
         if (r0 + stride < a.T) fetch(r0 + stride, next);           // under this row's arithmetic
-        const unsigned sel = gt_select<L, NV, VEC>(z, a.top_k);
-        rows += gt_softmax<L, NV>(z) ? 1 : 0;
+        unsigned key[NV];
+        float largest;
+        const unsigned floor_key = gt_select<L, NV, VEC>(z, a.top_k, key, largest);
+        rows += gt_softmax_at<L, NV>(z, largest) ? 1 : 0;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             ps[v] += z[v];
-            cn[v] += (sel >> v) & 1;
+            cn[v] += key[v] >= floor_key ? 1 : 0;
             z[v] = next[v];
         }
     }
@@ -322,34 +357,38 @@ __global__ __launch_bounds__(GT_NT) void gate_stats_kernel(GateArgs a, float* __
     if (threadIdx.x == 0) part_n[blockIdx.x] = (sn[0] + sn[1]) + (sn[2] + sn[3]);
 }
 
-// the workgroups' rows summed: 16 experts per workgroup, 16 threads each, float64, fixed order
-__global__ __launch_bounds__(256) void gate_reduce_kernel(const float* __restrict__ part_p, const int* __restrict__ part_c,
+// the workgroups' rows summed: 16 experts per workgroup, 64 threads each, float64, fixed order
+__global__ __launch_bounds__(1024) void gate_reduce_kernel(const float* __restrict__ part_p, const int* __restrict__ part_c,
                                                           const int* __restrict__ part_n, int nb, int E, int* __restrict__ counts,
                                                           float* __restrict__ mean_probs, int* __restrict__ n_valid) {
-    __shared__ double sp[16][17];
-    __shared__ int sc[16][17], sn[4];
+    __shared__ double sp[64][17];
+    __shared__ int sc[64][17], sn[16];
     const int x = threadIdx.x & 15, y = threadIdx.x >> 4, e = blockIdx.x * 16 + x;
     int n = 0;
-    for (int b = threadIdx.x; b < nb; b += 256) n += part_n[b];
+    for (int b = threadIdx.x; b < nb; b += 1024) n += part_n[b];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
     if ((threadIdx.x & 63) == 0) sn[threadIdx.x >> 6] = n;
     double p = 0.0;
     int c = 0;
-    if (e < E)
-        for (int b = y; b < nb; b += 16) {
+    if (e < E) {
+#pragma unroll 4
+        for (int b = y; b < nb; b += 64) {
             p += (double)part_p[(long)b * E + e];
             c += part_c[(long)b * E + e];
         }
+    }
     sp[y][x] = p;
     sc[y][x] = c;
     __syncthreads();
-    n = (sn[0] + sn[1]) + (sn[2] + sn[3]);
+    n = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) n += sn[i];
     if (y == 0 && e < E) {
         p = 0.0;
         c = 0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
+#pragma unroll 16
+        for (int i = 0; i < 64; ++i) {
             p += sp[i][x];
             c += sc[i][x];
         }
@@ -381,24 +420,70 @@ __global__ __launch_bounds__(64) void gate_loss_kernel(const int* __restrict__ c
     if (threadIdx.x == 0) loss[0] = v;
 }
 
+// few partial rows (nb E <= GT_SMALL_PARTIALS): every workgroup of the gradient sums them itself, in the same order, which saves
+// the launch in between
+constexpr int GT_SMALL_PARTIALS = 2048;
+struct GatePartials { const float* p; const int* c; const int* n; int nb; };
+
 // sweep 2.  Rows in the opposite order of sweep 1: what that read last is still in the cache behind the L2s.
-template <typename T, int L, int NV, int VEC>
-__global__ __launch_bounds__(GT_NT) void gate_grad_kernel(GateArgs a, const int* __restrict__ counts,
-                                                          const float* __restrict__ mean_probs, const int* __restrict__ n_valid,
+// REDUCE: counts, mean_probs and n_valid come from the partial rows (and are written, by workgroup 0) instead of from memory.
+template <typename T, int L, int NV, int VEC, bool REDUCE>
+__global__ __launch_bounds__(GT_NT) void gate_grad_kernel(GateArgs a, GatePartials parts, int* __restrict__ counts,
+                                                          float* __restrict__ mean_probs, int* __restrict__ n_valid,
                                                           const float* __restrict__ g_loss, const float* __restrict__ g_mean,
                                                           float* __restrict__ loss, T* __restrict__ grad) {
     constexpr int G = 64 / L;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & (L - 1);
-    const int n = n_valid[0];
+    __shared__ int s_count[REDUCE ? L * NV : 1], s_n[REDUCE ? GT_NT / 64 : 1];
+    __shared__ float s_mean[REDUCE ? L * NV : 1];
+    const int* count = counts;
+    const float* mean = mean_probs;
+    int n;
+    if constexpr (REDUCE) {
+        n = 0;
+        for (int b = threadIdx.x; b < parts.nb; b += GT_NT) n += parts.n[b];
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+        if (lane == 0) s_n[wave] = n;
+        __syncthreads();
+        n = 0;
+#pragma unroll
+        for (int i = 0; i < GT_NT / 64; ++i) n += s_n[i];
+        for (int e = wave; e < a.E; e += GT_NT / 64) {
+            double p = 0.0;
+            int c = 0;
+            for (int b = lane; b < parts.nb; b += 64) {
+                p += (double)parts.p[(long)b * a.E + e];
+                c += parts.c[(long)b * a.E + e];
+            }
+            p = wave_sum(p);
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
+            if (lane == 0) {
+                s_count[e] = c;
+                s_mean[e] = n > 0 ? (float)(p / (double)n) : 0.0f;
+                if (blockIdx.x == 0) {
+                    counts[e] = c;
+                    mean_probs[e] = s_mean[e];
+                }
+            }
+        }
+        if (blockIdx.x == 0 && threadIdx.x == 0) n_valid[0] = n;
+        __syncthreads();
+        count = s_count;
+        mean = s_mean;
+    } else {
+        n = n_valid[0];
+    }
     double count_mean;
-    const float value = gt_loss(counts, mean_probs, n, a.E, a.top_k, count_mean);
+    const float value = gt_loss(count, mean, n, a.E, a.top_k, count_mean);
     if (loss && blockIdx.x == 0 && threadIdx.x == 0) loss[0] = value;
     const float gl = g_loss ? g_loss[0] : 1.0f;
     float w[NV];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         const int e = GateMap<L, NV, VEC>::at(l, v);
-        w[v] = e < a.E ? gt_weight(counts[e], count_mean, n, a.E, a.top_k, gl, g_mean ? g_mean[e] : 0.0f) : 0.0f;
+        w[v] = e < a.E ? gt_weight(count[e], count_mean, n, a.E, a.top_k, gl, g_mean ? g_mean[e] : 0.0f) : 0.0f;
     }
     const long per = (long)gridDim.x * (GT_NT / 64) * G;
     const long mine = ((long)blockIdx.x * (GT_NT / 64) + wave) * G;
@@ -456,7 +541,7 @@ __global__ __launch_bounds__(GT_ONE_NT) void gate_one_kernel(GateArgs a, float* 
     const float value = gt_loss(count, mean, n, a.E, a.top_k, count_mean);
     if (threadIdx.x == 0) {
         loss[0] = value;
-        n_valid[0] = n;
+        if (n_valid) n_valid[0] = n;
     }
     if (!grad) return;
     float w[NV];
@@ -472,9 +557,9 @@ __global__ __launch_bounds__(GT_ONE_NT) void gate_one_kernel(GateArgs a, float* 
 constexpr int GT_BLOCKS = 1024;                  // workgroups of a sweep: four per CU
 constexpr int GT_MAX_EXPERTS = 1024;
 
-static int gt_lanes(int E) {                     // lanes per row, eight values each
+static int gt_lanes(int E) {                     // lanes per row: eight values each up to 128 experts, sixteen above
     int l = 1;
-    while (l < 64 && l * 8 < E) l <<= 1;
+    while (l * (E > 128 ? 16 : 8) < E) l <<= 1;
     return l;
 }
 static int gt_blocks(long T, int E) {
@@ -506,10 +591,17 @@ static int gt_run(const GateArgs& a, const GateWork& w, const GateOut& o, bool s
         return 0;
     }
     const int nb = gt_blocks(a.T, a.E);
+    const GatePartials parts = {w.p, w.c, w.n, nb};
     if (stats) {
         hipLaunchKernelGGL((gate_stats_kernel<T, L, NV, VEC>), dim3(nb), dim3(GT_NT), 0, st, a, w.p, w.c, w.n);
         MV_LAUNCH_CHECK("gate_stats_kernel");
-        hipLaunchKernelGGL(gate_reduce_kernel, dim3((a.E + 15) / 16), dim3(256), 0, st, (const float*)w.p, (const int*)w.c,
+        if (o.grad && (long)nb * a.E <= GT_SMALL_PARTIALS) {
+            hipLaunchKernelGGL((gate_grad_kernel<T, L, NV, VEC, true>), dim3(nb), dim3(GT_NT), 0, st, a, parts, o.counts, o.mean_probs,
+                               o.n_valid, o.g_loss, o.g_mean, o.loss, (T*)o.grad);
+            MV_LAUNCH_CHECK("gate_grad_kernel");
+            return 0;
+        }
+        hipLaunchKernelGGL(gate_reduce_kernel, dim3((a.E + 15) / 16), dim3(1024), 0, st, (const float*)w.p, (const int*)w.c,
                            (const int*)w.n, nb, a.E, o.counts, o.mean_probs, o.n_valid);
         MV_LAUNCH_CHECK("gate_reduce_kernel");
         if (!o.grad) {
@@ -519,23 +611,27 @@ static int gt_run(const GateArgs& a, const GateWork& w, const GateOut& o, bool s
             return 0;
         }
     }
-    hipLaunchKernelGGL((gate_grad_kernel<T, L, NV, VEC>), dim3(nb), dim3(GT_NT), 0, st, a, (const int*)o.counts,
-                       (const float*)o.mean_probs, (const int*)o.n_valid, o.g_loss, o.g_mean, stats ? o.loss : nullptr, (T*)o.grad);
+    hipLaunchKernelGGL((gate_grad_kernel<T, L, NV, VEC, false>), dim3(nb), dim3(GT_NT), 0, st, a, parts, o.counts, o.mean_probs, o.n_valid,
+                       o.g_loss, o.g_mean, stats ? o.loss : nullptr, (T*)o.grad);
     MV_LAUNCH_CHECK("gate_grad_kernel");
     return 0;
 }
 
 template <typename T, int VEC>
 static int gt_dispatch_lanes(const GateArgs& a, const GateWork& w, const GateOut& o, bool stats, hipStream_t st) {
-    if (a.E > 512) return gt_run<T, 64, 16, VEC>(a, w, o, stats, st);
+    if (a.E > 128) {
+        switch (gt_lanes(a.E)) {
+            case 16: return gt_run<T, 16, 16, VEC>(a, w, o, stats, st);
+            case 32: return gt_run<T, 32, 16, VEC>(a, w, o, stats, st);
+            default: return gt_run<T, 64, 16, VEC>(a, w, o, stats, st);
+        }
+    }
     switch (gt_lanes(a.E)) {
         case 1: return gt_run<T, 1, 8, VEC>(a, w, o, stats, st);
         case 2: return gt_run<T, 2, 8, VEC>(a, w, o, stats, st);
         case 4: return gt_run<T, 4, 8, VEC>(a, w, o, stats, st);
         case 8: return gt_run<T, 8, 8, VEC>(a, w, o, stats, st);
-        case 16: return gt_run<T, 16, 8, VEC>(a, w, o, stats, st);
-        case 32: return gt_run<T, 32, 8, VEC>(a, w, o, stats, st);
-        default: return gt_run<T, 64, 8, VEC>(a, w, o, stats, st);
+        default: return gt_run<T, 16, 8, VEC>(a, w, o, stats, st);
     }
 }
 template <typename T>
@@ -560,7 +656,7 @@ using namespace mdnvae;
 
 extern "C" size_t mdnvae_gate_balance_workspace_bytes(long T, int E) {
     if (T < 1 || E < 1 || E > GT_MAX_EXPERTS || gt_one(T, E)) return 0;
-    return (size_t)gt_blocks(T, E) * ((size_t)E * 8 + 4);
+    return (size_t)gt_blocks(T, E) * ((size_t)E * 8 + 4) + 4;
 }
 
 extern "C" int mdnvae_gate_balance(const void* logits, const unsigned char* valid, long T, int E, int top_k, int dtype, void* workspace,
@@ -568,7 +664,7 @@ extern "C" int mdnvae_gate_balance(const void* logits, const unsigned char* vali
                                    void* stream) {
     const int bad = gt_check("mdnvae_gate_balance", logits, T, E, top_k, dtype);
     if (bad) return bad;
-    MV_REQUIRE(loss && counts && mean_probs && n_valid, E_ARG, "mdnvae_gate_balance: null output");
+    MV_REQUIRE(loss && counts && mean_probs, E_ARG, "mdnvae_gate_balance: null output");
     const size_t need = mdnvae_gate_balance_workspace_bytes(T, E);
     MV_REQUIRE(workspace_bytes >= need && (workspace || need == 0), E_ARG, "mdnvae_gate_balance: workspace of %zu bytes, %zu are needed",
                workspace_bytes, need);
@@ -577,6 +673,7 @@ extern "C" int mdnvae_gate_balance(const void* logits, const unsigned char* vali
     const size_t nb = need ? (size_t)gt_blocks(T, E) : 0;
     float* p = static_cast<float*>(workspace);
     const GateWork w = {p, reinterpret_cast<int*>(p + nb * E), reinterpret_cast<int*>(p + 2 * nb * E)};
+    if (!n_valid && need) n_valid = reinterpret_cast<int*>(p + 2 * nb * E) + nb;
     const GateOut o = {loss, counts, mean_probs, n_valid, grad, nullptr, nullptr};
     return dtype == MDNVAE_F32 ? gt_dispatch<float>(a, w, o, true, (hipStream_t)stream)
                                : gt_dispatch<__bf16>(a, w, o, true, (hipStream_t)stream);

@@ -22,6 +22,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <cstdlib>
 #include "common.h"
 #include "../../include/mdnvae_hip.h"
 
@@ -595,12 +596,6 @@ __global__ __launch_bounds__(256) void mu_reduce_kernel(MuTab tab, char* __restr
     mu_emit_block<TERMS == 3 ? 2 : 1, false>(acc, A, MuOld(), ge.mp >> 4, rb, cb, ti != tj, sc, smem + wid * 4096);
 }
 
-// where a finished result goes: out = v, or the parameter step p <- decay p - lr_scale v (one rounding to T)
-template <typename T>
-__device__ __forceinline__ void mu_finish(T* p, long i, float v, float decay, float lr_scale, bool step) {
-    p[i] = (T)(step ? decay * (float)p[i] - lr_scale * v : v);
-}
-
 // STEP: D rows = 128 (64) columns n of X, D columns = rows m, so that a lane's four consecutive rows are consecutive in X's
 // tiles.  LAST: the result leaves in the caller's layout and type.
 template <typename T, int TILE, int TERMS, bool LAST>
@@ -699,194 +694,218 @@ __global__ __launch_bounds__(256) void mu_step_kernel(MuTab tab, int total, MuPt
 
 // ---- small matrices: the whole step in one workgroup ----------------------------------------------------------------------
 // X and A in parts fit LDS (mp np + mp mp <= 38912 entries, mp and np multiples of 32): norm, all iterations and the
-// parameter step in one launch, one matrix per workgroup of 16 waves.  A 32 x 32 block of a product belongs to one
-// wave; its registers are held until a barrier says that everybody has read what they overwrite.
+// parameter step in one launch, one matrix per workgroup of up to 16 waves.  A 32 x 32 block of a product belongs to one
+// wave; its registers are held until a barrier says that everybody has read what they overwrite.  Always both parts:
+// such a matrix is bound by latencies and barriers, not by its products.
 constexpr int MU_SMALL_ENTRIES = 38912;
 constexpr int MU_SMALL_NT = 1024;
 constexpr int MU_SMALL_BLOCKS = (MU_SMALL_ENTRIES / 1024 + 15) / 16;      // 32 x 32 blocks of X per wave
-constexpr int MU_SMALL_CHUNKS = (MU_SMALL_ENTRIES / 8 + MU_SMALL_NT - 1) / MU_SMALL_NT;
 
 struct MuSteps {                                   // per iteration: the three products' scales
     int steps;
     MuScale gram[MDNVAE_MUON_MAX_STEPS], poly[MDNVAE_MUON_MAX_STEPS], step[MDNVAE_MUON_MAX_STEPS];
 };
 
-template <typename T, int TERMS>
+// acc = 32 rows x 32 columns over K (even) k steps: operand rows at `rows` (read along a row, or, TR, down the columns of X
+// whose tile rows are `pitch` bytes apart), the next step's operands on their way while this one's are multiplied
+template <bool TR>
+__device__ __forceinline__ void mu_small_product(const char* rows, const char* cols, int K, long pitch, const MuLane& ln, int tr_extra,
+                                                 mu_acc& acc) {
+    mu_h8 r[2][2], c[2][2];
+    auto load = [&](int set, int ks) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            c[set][s] = *reinterpret_cast<const mu_h8*>(cols + ks * MU_STEP + s * MU_FRAG + ln.direct);
+            if constexpr (TR) r[set][s] = mu_tr(rows + (ks >> 1) * pitch + (ks & 1) * 512 + s * MU_FRAG + tr_extra + ln.tr);
+            else r[set][s] = *reinterpret_cast<const mu_h8*>(rows + ks * MU_STEP + s * MU_FRAG + ln.direct);
+        }
+    };
+    auto multiply = [&](int set) {
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[set][1], c[set][0], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[set][0], c[set][1], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[set][0], c[set][0], acc, 0, 0, 0);
+    };
+#pragma unroll
+    for (int k = 0; k < 16; ++k) acc[k] = 0.0f;
+    load(0, 0);
+    for (int ks = 0; ks < K; ks += 2) {
+        load(1, ks + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(0);
+        if (ks + 2 < K) load(0, ks + 2);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(1);
+    }
+}
+
+// BL: blocks of X per wave
+template <typename T, int BL>
 __global__ __launch_bounds__(MU_SMALL_NT) void mu_small_kernel(MuTab tab, MuPtrs ptrs, MuMom mm, float eps, float x_scale, MuSteps st,
                                                                float decay, int is_step) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     __shared__ double red[MU_SMALL_NT / 64];
-    constexpr int NP = TERMS == 3 ? 2 : 1;
     const int e = mu_entry(tab, blockIdx.x);
     const MuGeo& ge = tab.e[e];
-    const long len = (long)ge.m * ge.n;
-    const long mat = blockIdx.x - tab.start[e];
+    const int m_valid = ge.m, n_valid = ge.n, trans = ge.trans;
+    const long len = (long)m_valid * n_valid, mat = blockIdx.x - tab.start[e];
     const T* g = static_cast<const T*>(ptrs.g[e]) + mat * len;
     float* mom = ptrs.mom[e];
     T* out = static_cast<T*>(ptrs.p[e]) + mat * len;
     const int NS = ge.np >> 4, KS = ge.mp >> 4, MB = ge.mp >> 5, NB = ge.np >> 5;
     char* X = smem;
     char* A = smem + 4 * ge.mp * ge.np;
-    const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, nt = blockDim.x, waves = nt >> 6;
     const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const MuLane ln = mu_lane(lane);
 
-    {   // G (momentum) in, eight columns of a row per chunk
-        float u[MU_SMALL_CHUNKS][8];
+    {   // G (momentum) in, eight columns of a row per chunk; every load is issued whether its entry exists or not (entry 0
+        // stands in).  Until the norm is known a chunk waits as eight floats in the 32 bytes its two parts will have.
         const int per_row = ge.np >> 3, chunks = ge.mp * per_row;
+        auto place = [&](int r, int c8) { return X + ((r >> 5) * NS + (c8 >> 1)) * MU_STEP + mu_at(r & 31, c8 & 1); };
+        const float m0 = mom ? mm.mu * mom[0] + (float)g[0] : 0.0f;
         double s = 0.0;
-#pragma unroll
-        for (int c = 0; c < MU_SMALL_CHUNKS; ++c) {
-            const int ch = tid + c * MU_SMALL_NT;
-            const int r = ch / per_row, c0 = (ch - r * per_row) * 8;
+#pragma unroll 2
+        for (int ch = tid; ch < chunks; ch += nt) {
+            const int r = ch / per_row, c8 = ch - r * per_row;
+            int at[8];                                      // within the matrix: fits an int
+            float u[8], m[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                u[c][k] = 0.0f;
-                if (ch < chunks && r < ge.m && c0 + k < ge.n) {
-                    u[c][k] = mu_update(g, mom, ge.trans ? (long)(c0 + k) * ge.m + r : (long)r * ge.n + c0 + k, mm, true);
-                    s += (double)u[c][k] * (double)u[c][k];
+                const int c = c8 * 8 + k;
+                at[k] = r < m_valid && c < n_valid ? (trans ? c * m_valid + r : r * n_valid + c) : -1;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) u[k] = (float)g[max(at[k], 0)];
+            if (mom) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) m[k] = mom[max(at[k], 0)];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    m[k] = mm.mu * m[k] + u[k];
+                    u[k] = mm.nesterov ? u[k] + mm.mu * m[k] : m[k];
+                    if (at[k] > 0) mom[at[k]] = m[k];       // entry 0: once everybody has read it
                 }
             }
+            mu_f4 lo4, hi4;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if (at[k] < 0) u[k] = 0.0f;
+                s += (double)u[k] * (double)u[k];
+                if (k < 4) lo4[k] = u[k];
+                else hi4[k - 4] = u[k];
+            }
+            *reinterpret_cast<mu_f4*>(place(r, c8)) = lo4;
+            *reinterpret_cast<mu_f4*>(place(r, c8) + MU_FRAG) = hi4;
         }
         s = wave_sum(s);
         if (lane == 0) red[wid] = s;
         __syncthreads();
+        if (mom && tid == 0) mom[0] = m0;
         s = 0.0;
-#pragma unroll
-        for (int i = 0; i < MU_SMALL_NT / 64; ++i) s += red[i];
+        for (int i = 0; i < waves; ++i) s += red[i];
         const double inv = mu_inv_norm(s, eps, x_scale);
+        for (int ch = tid; ch < chunks; ch += nt) {         // the thread's own chunks
+            const int r = ch / per_row, c8 = ch - r * per_row;
+            char* dst = place(r, c8);
+            const mu_f4 lo4 = *reinterpret_cast<const mu_f4*>(dst), hi4 = *reinterpret_cast<const mu_f4*>(dst + MU_FRAG);
+            mu_h8 hi, lo;
 #pragma unroll
-        for (int c = 0; c < MU_SMALL_CHUNKS; ++c) {
-            const int ch = tid + c * MU_SMALL_NT;
-            if (ch < chunks) {
-                const int r = ch / per_row, c8 = ch - r * per_row;
-                mu_h8 hi, lo;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    _Float16 a, b;
-                    mu_parts((float)((double)u[c][k] * inv), a, b);
-                    hi[k] = a;
-                    lo[k] = b;
-                }
-                char* dst = X + ((r >> 5) * NS + (c8 >> 1)) * MU_STEP + mu_at(r & 31, c8 & 1);
-                *reinterpret_cast<mu_h8*>(dst) = hi;
-                *reinterpret_cast<mu_h8*>(dst + MU_FRAG) = lo;
+            for (int k = 0; k < 8; ++k) {
+                _Float16 a, b;
+                mu_parts((float)((double)(k < 4 ? lo4[k & 3] : hi4[k & 3]) * inv), a, b);
+                hi[k] = a;
+                lo[k] = b;
             }
+            *reinterpret_cast<mu_h8*>(dst) = hi;
+            *reinterpret_cast<mu_h8*>(dst + MU_FRAG) = lo;
         }
         __syncthreads();
     }
 
-    // one 32 x 32 block: rows of `rows` (tile rb) times rows of `cols` (tile cb), or the columns of X (TR)
-    auto mfma = [&](const mu_h8 (&r)[NP], const mu_h8 (&c)[NP], mu_acc& acc) {
-        if constexpr (TERMS == 3) {
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[1], c[0], acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[0], c[1], acc, 0, 0, 0);
-        }
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[0], c[0], acc, 0, 0, 0);
+    auto put = [&](char* at, const mu_acc& v, int q) {
+        const float four[4] = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+        mu_put<2>(at, four);
     };
-    auto zero = [](mu_acc& acc) {
-#pragma unroll
-        for (int k = 0; k < 16; ++k) acc[k] = 0.0f;
-    };
-    auto product = [&](const char* rows, const char* cols, int K, mu_acc& acc) {
-        zero(acc);
-        for (int ks = 0; ks < K; ++ks) {
-            mu_h8 r[NP], c[NP];
-#pragma unroll
-            for (int s = 0; s < NP; ++s) {
-                r[s] = *reinterpret_cast<const mu_h8*>(rows + ks * MU_STEP + s * MU_FRAG + ln.direct);
-                c[s] = *reinterpret_cast<const mu_h8*>(cols + ks * MU_STEP + s * MU_FRAG + ln.direct);
-            }
-            mfma(r, c, acc);
-        }
-    };
+    const int rb = wid / MB, cb = wid - rb * MB;
+    const bool mine = wid < MB * MB;                        // at most 16 blocks of A: one per wave
+    // the two n steps of a block of X are MU_STEP apart here, not 512 bytes
+    const int tr_extra = ((lane >> 4) & 1) * (MU_STEP - 512);
     for (int it = 0; it < st.steps; ++it) {
-        // A = X X^T (at most 16 blocks: one per wave)
+        // A = X X^T
         mu_acc acc;
-        const int rb = wid / MB, cb = wid - rb * MB;
-        const bool mine = wid < MB * MB;
         if (mine) {
-            product(X + rb * NS * MU_STEP, X + cb * NS * MU_STEP, NS, acc);
+            mu_small_product<false>(X + rb * NS * MU_STEP, X + cb * NS * MU_STEP, NS, 0, ln, 0, acc);
+            const float f = st.gram[it].f_acc;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                float v[4];
+            for (int k = 0; k < 16; ++k) acc[k] *= f;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] = acc[4 * q + k] * st.gram[it].f_acc;
-                mu_put<NP>(A + mu_block_at(cb, KS, rb * 32, q, lane), v);
-            }
+            for (int q = 0; q < 4; ++q) put(A + mu_block_at(cb, KS, rb * 32, q, lane), acc, q);
         }
         __syncthreads();
         // B = b A + c A^2, over A
-        float v4[4][4];
         if (mine) {
-            product(A + rb * KS * MU_STEP, A + cb * KS * MU_STEP, KS, acc);
+            mu_small_product<false>(A + rb * KS * MU_STEP, A + cb * KS * MU_STEP, KS, 0, ln, 0, acc);
             MuOld old;
-            mu_load_block<NP>(old, A, cb, KS, rb * 32, lane);
+            mu_load_block<2>(old, A, cb, KS, rb * 32, lane);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v4[q][k] = acc[4 * q + k] * st.poly[it].f_acc + mu_old<NP>(old, q, k) * st.poly[it].f_add;
-            }
+            for (int k = 0; k < 16; ++k) acc[k] = acc[k] * st.poly[it].f_acc + mu_old<2>(old, k >> 2, k & 3) * st.poly[it].f_add;
         }
         __syncthreads();
         if (mine) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) mu_put<NP>(A + mu_block_at(cb, KS, rb * 32, q, lane), v4[q]);
+            for (int q = 0; q < 4; ++q) put(A + mu_block_at(cb, KS, rb * 32, q, lane), acc, q);
         }
         __syncthreads();
         // X <- a X + B X
-        mu_acc y[MU_SMALL_BLOCKS];
+        mu_acc y[BL];
 #pragma unroll
-        for (int b = 0; b < MU_SMALL_BLOCKS; ++b) {
-            const int id = wid + b * (MU_SMALL_NT / 64);
+        for (int b = 0; b < BL; ++b) {
+            const int id = wid + b * waves;
             if (id < MB * NB) {
                 const int nb = id / MB, mb = id - nb * MB;
-                zero(y[b]);
-                for (int ks = 0; ks < KS; ++ks) {
-                    mu_h8 r[NP], c[NP];
-#pragma unroll
-                    for (int s = 0; s < NP; ++s) {
-                        c[s] = *reinterpret_cast<const mu_h8*>(A + (mb * KS + ks) * MU_STEP + s * MU_FRAG + ln.direct);
-                        // the two n steps of a block are 2 KiB apart here, not 512 bytes
-                        const char* t = X + ((ks >> 1) * NS + nb * 2) * MU_STEP + s * MU_FRAG + (ks & 1) * 512 +
-                                        ((lane >> 4) & 1) * (MU_STEP - 512);
-                        r[s] = mu_tr(t + ln.tr);
-                    }
-                    mfma(r, c, y[b]);
-                }
-                MuOld old;
-                mu_load_block<2>(old, X, mb, NS, nb * 32, lane);
-#pragma unroll
-                for (int k = 0; k < 16; ++k)
-                    y[b][k] = y[b][k] * st.step[it].f_acc + mu_old<2>(old, k >> 2, k & 3) * st.step[it].f_add;
+                mu_small_product<true>(X + nb * 2 * MU_STEP, A + mb * KS * MU_STEP, KS, (long)NS * MU_STEP, ln, tr_extra, y[b]);
             }
+            __builtin_amdgcn_sched_barrier(0);              // a block's operands in registers at a time
         }
         __syncthreads();
         const bool last = it + 1 == st.steps;
 #pragma unroll
-        for (int b = 0; b < MU_SMALL_BLOCKS; ++b) {
-            const int id = wid + b * (MU_SMALL_NT / 64);
+        for (int b = 0; b < BL; ++b) {
+            const int id = wid + b * waves;
             if (id < MB * NB) {
                 const int nb = id / MB, mb = id - nb * MB;
+                MuOld old;                                  // what the block replaces is where it goes
+                mu_load_block<2>(old, X, mb, NS, nb * 32, lane);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    float v[4];
+                for (int k = 0; k < 16; ++k)
+                    y[b][k] = y[b][k] * st.step[it].f_acc + mu_old<2>(old, k >> 2, k & 3) * st.step[it].f_add;
+                if (!last) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) v[k] = y[b][4 * q + k];
-                    if (!last) {
-                        mu_put<2>(X + mu_block_at(mb, NS, nb * 32, q, lane), v);
-                    } else {
-                        const int m = mb * 32 + (lane & 31), n = nb * 32 + 8 * q + 4 * h;
-                        if (m < ge.m) {
+                    for (int q = 0; q < 4; ++q) put(X + mu_block_at(mb, NS, nb * 32, q, lane), y[b], q);
+                } else {
+                    const int m = mb * 32 + (lane & 31), n = nb * 32 + 4 * h;
+                    const int left = m < m_valid ? n_valid - n : 0;                 // columns from n on that exist
+                    const int step = trans ? m_valid : 1;
+                    T* dst = out + (trans ? n * m_valid + m : m * n_valid + n);
+                    const float lr_scale = ptrs.lr_scale[e];
+                    T p[16];
+                    if (is_step) {
 #pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                if (n + k < ge.n)
-                                    mu_finish(out, ge.trans ? (long)(n + k) * ge.m + m : (long)m * ge.n + n + k, v[k], decay,
-                                              ptrs.lr_scale[e], is_step != 0);
+                        for (int k = 0; k < 16; ++k) {
+                            const int c = 8 * (k >> 2) + (k & 3);
+                            p[k] = c < left ? dst[c * step] : (T)0.0f;
                         }
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) y[b][k] = decay * (float)p[k] - lr_scale * y[b][k];
+                    }
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const int c = 8 * (k >> 2) + (k & 3);
+                        if (c < left) dst[c * step] = (T)y[b][k];
                     }
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
         __syncthreads();
     }
@@ -962,6 +981,9 @@ static bool mu_small(const MuJob& j) {
 #define MU_TMIN 16
 #endif
 constexpr int MU_TARGET_WGS = MU_TW;               // two workgroups per CU: what the splits of X X^T aim at
+#ifndef MU_T128
+#define MU_T128 256
+#endif
 constexpr long MU_PASS_BYTES = 1L << 30;         // workspace beyond which a batch is run in several passes
 constexpr long MU_MAX_SIDE = 65536, MU_MAX_LONG = 1L << 24, MU_MAX_ENTRIES = 1L << 36;
 
@@ -984,7 +1006,7 @@ static void mu_plan(const MuJob* jobs, int n, MuPlan& pl) {
         const long m = std::min(jobs[i].rows, jobs[i].cols), c = std::max(jobs[i].rows, jobs[i].cols);
         t128 += jobs[i].count * (mu_up(m, 128) / 128) * (mu_up(c, 128) / 128);
     }
-    const int tile = t128 >= 256 ? 128 : 64;
+    const int tile = t128 >= MU_T128 ? 128 : 64;
     pl.tile = tile;
     pl.n = n;
     long work = 0;
@@ -1047,13 +1069,13 @@ static int mu_starts(const MuPlan& pl, int* start, F per_matrix) {
     return (int)at;
 }
 
-template <typename T, int TERMS>
+template <typename T>
 static int mu_run_small(const MuJob* jobs, int n, const MuRun& r) {
     MuTab tab;
     MuPtrs pt;
     mu_pointers(jobs, n, pt);
     tab.n = n;
-    long at = 0, most = 0;
+    long at = 0, most = 0, blocks = 4;
     for (int i = 0; i <= MU_MAX; ++i) tab.start[i] = INT_MAX;
     for (int i = 0; i < n; ++i) {
         MuGeo& g = tab.e[i];
@@ -1068,13 +1090,15 @@ static int mu_run_small(const MuJob* jobs, int n, const MuRun& r) {
         tab.start[i] = (int)at;
         at += jobs[i].count;
         most = std::max(most, 4L * g.mp * (g.np + g.mp));
+        blocks = std::max(blocks, (long)(g.mp / 32) * (g.np / 32));
         MV_REQUIRE(at <= (1L << 30), E_SHAPE, "mdnvae_orthogonalize: too many matrices for one launch");
     }
-    auto kern = mu_small_kernel<T, TERMS>;
+    // one block of X per wave (up to 128 x 128) keeps everything in registers; with three some wait in scratch memory
+    auto kern = blocks <= MU_SMALL_NT / 64 ? mu_small_kernel<T, 1> : mu_small_kernel<T, MU_SMALL_BLOCKS>;
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
                                              4 * MU_SMALL_ENTRIES);
     MV_REQUIRE(e == hipSuccess, (int)e, "mu_small_kernel: cannot raise the LDS limit: %s", hipGetErrorString(e));
-    hipLaunchKernelGGL(kern, dim3((unsigned)at), dim3(MU_SMALL_NT), (size_t)most, r.stream, tab, pt, r.mm, r.co.eps, r.x0_scale, r.st,
+    hipLaunchKernelGGL(kern, dim3((unsigned)at), dim3((unsigned)std::min((long)MU_SMALL_NT, blocks * 64)), (size_t)most, r.stream, tab, pt, r.mm, r.co.eps, r.x0_scale, r.st,
                        r.decay, r.is_step);
     MV_LAUNCH_CHECK("mu_small_kernel");
     return 0;
@@ -1142,7 +1166,7 @@ static int mu_run_tiled(const MuJob* jobs, const MuPlan& pl, const MuRun& r, cha
 template <typename T, int TERMS>
 static int mu_run(const MuJob* jobs, int n, bool small, const MuRun& r, char* ws) {
     if (n == 0) return 0;
-    if (small) return mu_run_small<T, TERMS>(jobs, n, r);
+    if (small) return mu_run_small<T>(jobs, n, r);
     MuPlan pl;
     mu_plan(jobs, n, pl);
     return pl.tile == 128 ? mu_run_tiled<T, TERMS, 128>(jobs, pl, r, ws) : mu_run_tiled<T, TERMS, 64>(jobs, pl, r, ws);
@@ -1247,6 +1271,34 @@ static int mu_groups(const long* rows, const long* cols, int count, F f) {
     return 0;
 }
 
+// Whether what a step writes (parameters, momenta) overlaps anything else it touches; -1 without memory for the check.
+struct MuSpan { uintptr_t lo, hi; int written; };
+static int mu_overlap(void* const* params, const void* const* grads, float* const* momenta, const long* rows, const long* cols, int count,
+                      int size) {
+    MuSpan* s = static_cast<MuSpan*>(std::malloc((size_t)count * 3 * sizeof(MuSpan)));
+    if (!s) return -1;
+    long n = 0;
+    for (int i = 0; i < count; ++i) {
+        const uintptr_t len = (uintptr_t)rows[i] * (uintptr_t)cols[i];
+        if (!len) continue;
+        const void* at[3] = {params[i], grads[i], momenta[i]};
+        for (int k = 0; k < 3; ++k) {
+            const uintptr_t lo = reinterpret_cast<uintptr_t>(at[k]);
+            s[n++] = {lo, lo + len * (k == 2 ? 4 : size), k != 1};
+        }
+    }
+    std::sort(s, s + n, [](const MuSpan& a, const MuSpan& b) { return a.lo < b.lo; });
+    uintptr_t end = 0, end_written = 0;
+    int bad = 0;
+    for (long i = 0; i < n && !bad; ++i) {
+        bad = s[i].lo < (s[i].written ? end : end_written);
+        end = std::max(end, s[i].hi);
+        if (s[i].written) end_written = std::max(end_written, s[i].hi);
+    }
+    std::free(s);
+    return bad;
+}
+
 extern "C" size_t mdnvae_muon_workspace_bytes(const long* rows, const long* cols, int count) {
     if (count < 1 || !rows || !cols) return 0;
     for (int i = 0; i < count; ++i)
@@ -1284,6 +1336,9 @@ extern "C" int mdnvae_muon_step(void* const* params, const void* const* grads, f
                    cols[i]);
         MV_REQUIRE(params[i] && grads[i] && momenta[i], E_ARG, "mdnvae_muon_step: null pointer of matrix %d", i);
     }
+    const int overlap = mu_overlap(params, grads, momenta, rows, cols, count, dtype == MDNVAE_F32 ? 4 : 2);
+    MV_REQUIRE(overlap >= 0, E_ARG, "mdnvae_muon_step: no host memory");
+    MV_REQUIRE(overlap == 0, E_ARG, "mdnvae_muon_step: a parameter or momentum overlaps another tensor of the step (in the list twice?)");
     const size_t need = mdnvae_muon_workspace_bytes(rows, cols, count);
     MV_REQUIRE(workspace_bytes >= need && (workspace || need == 0), E_ARG, "mdnvae_muon_step: workspace of %zu bytes, %zu are needed",
                workspace_bytes, need);

@@ -2001,6 +2001,14 @@ def _workspace(nbytes, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
+_HERE = contextlib.nullcontext()
+
+
+def _on(device):
+    """Launches go to the tensors' device and its current stream, whatever device is current."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
 def orthogonalize(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, arithmetic=None, out=None):
     """The nearest thing to an orthogonal matrix that `steps` Newton-Schulz steps reach from each matrix of x [..., m, n]
     (fp32 or bf16, contiguous): X = x / max(|x|_F, eps), then X <- a X + (b A + c A^2) X with A = X X^T (of the
@@ -2028,11 +2036,23 @@ def orthogonalize(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, arithmetic
     batch = x.numel() // (rows * cols)
     a, b, c = (float(v) for v in coefficients)
     lib = _lib.load()
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         ws = _workspace(lib.mdnvae_orthogonalize_workspace_bytes(batch, rows, cols), x.device)
         call("mdnvae_orthogonalize", xp, op, batch, rows, cols, dtype, int(steps), a, b, c, float(eps),
              _update_terms(arithmetic, x.dtype), None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), stream())
     return out
+
+
+def _refuse_muon(i, p, g, m, dtype, device):
+    for t, name, want in ((p, f"params[{i}]", dtype), (g, f"grads[{i}]", dtype), (m, f"momenta[{i}]", torch.float32)):
+        if t is None:
+            raise RuntimeError(f"muon_step: {name} is missing")
+        ptr(t.detach() if isinstance(t, torch.Tensor) else t, name, want)
+        if t.device != device:
+            raise RuntimeError(f"muon_step: {name} is on {t.device}, params[0] on {device}")
+    if p.dim() < 2:
+        raise RuntimeError(f"muon_step: params[{i}] {tuple(p.shape)} must have at least two dimensions")
+    raise RuntimeError(f"muon_step: params[{i}] {tuple(p.shape)} needs a gradient {tuple(g.shape)} and a momentum {tuple(m.shape)} of its shape")
 
 
 def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_decay=0.0, scale="shape", steps=5,
@@ -2051,33 +2071,24 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
         raise ValueError(f"scale {scale!r}: one of {list(UPDATE_SCALES)}")
     if not params:
         return
-    dtype, dev = _element_type(params[0], "params[0]"), params[0].device
-    n = len(params)
-    pp, gp, mp = (ctypes.c_void_p * n)(), (ctypes.c_void_p * n)(), (ctypes.c_void_p * n)()
+    etype, dt, dev, n = _element_type(params[0], "params[0]"), params[0].dtype, params[0].device, len(params)
     rows, cols = (ctypes.c_long * n)(), (ctypes.c_long * n)()
-    spans = []
     for i, (p, g, m) in enumerate(zip(params, grads, momenta)):
-        if not isinstance(p, torch.Tensor) or p.dim() < 2:
-            raise RuntimeError(f"muon_step: params[{i}] must be a tensor of at least two dimensions")
-        pp[i], gp[i] = ptr(p.detach(), f"params[{i}]", params[0].dtype), ptr(g, f"grads[{i}]", params[0].dtype)
-        mp[i] = ptr(m, f"momenta[{i}]", torch.float32)
-        if g is None or m is None or g.shape != p.shape or m.shape != p.shape:
-            raise RuntimeError(f"muon_step: params[{i}] {tuple(p.shape)} needs a gradient and a momentum of its shape")
-        if p.device != dev or g.device != dev or m.device != dev:
-            raise RuntimeError(f"muon_step: params[{i}], its gradient and its momentum must all be on {dev}")
-        rows[i] = p.shape[0]
-        cols[i] = p.numel() // p.shape[0] if p.numel() else 0
-        if p.numel():
-            spans += [(pp[i], p.numel() * p.element_size()), (mp[i], 4 * m.numel())]
-    spans.sort()
-    if any(a + size > b for (a, size), (b, _) in zip(spans, spans[1:])):
-        raise RuntimeError("muon_step: parameters and momenta must not overlap (is a tensor in the list twice?)")
+        shape = p.shape
+        if not (p.dtype == dt == g.dtype and m.dtype == torch.float32 and g.shape == shape == m.shape and len(shape) > 1
+                and p.device == dev == g.device and m.device == dev and p.is_contiguous() and g.is_contiguous() and m.is_contiguous()):
+            _refuse_muon(i, p, g, m, dt, dev)
+        rows[i] = shape[0]
+        cols[i] = shape[1] if len(shape) == 2 else shape[1:].numel()
+    ptr(params[0].detach(), "params[0]", dt)             # device memory: the others are where this one is
+    pointers = ctypes.c_void_p * n
+    pp, gp, mp = (pointers(*[t.data_ptr() for t in ts]) for ts in (params, grads, momenta))
     a, b, c = (float(v) for v in coefficients)
     lib = _lib.load()
-    with torch.cuda.device(dev):
+    with _on(dev):
         ws = _workspace(lib.mdnvae_muon_workspace_bytes(rows, cols, n), dev)
-        call("mdnvae_muon_step", pp, gp, mp, rows, cols, n, dtype, float(lr), float(momentum), int(bool(nesterov)), float(weight_decay),
-             UPDATE_SCALES[scale], int(steps), a, b, c, float(eps), _update_terms(arithmetic, params[0].dtype),
+        call("mdnvae_muon_step", pp, gp, mp, rows, cols, n, etype, float(lr), float(momentum), int(bool(nesterov)), float(weight_decay),
+             UPDATE_SCALES[scale], int(steps), a, b, c, float(eps), _update_terms(arithmetic, dt),
              None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), stream())
 
 
@@ -2093,15 +2104,15 @@ def _gate_call(logits, top_k, valid, want_grad):
     if valid is not None and (valid.shape != (T,) or valid.device != dev):
         raise RuntimeError(f"gate balance loss: valid {tuple(valid.shape)} on {valid.device} must be [{T}] on {dev}")
     lib = _lib.load()
-    with torch.cuda.device(dev):
+    with _on(dev):
         loss = torch.empty((), dtype=torch.float32, device=dev)
         counts = torch.empty(E, dtype=torch.int32, device=dev)
         mean_probs = torch.empty(E, dtype=torch.float32, device=dev)
-        n_valid = torch.empty(1, dtype=torch.int32, device=dev)
+        n_valid = None if want_grad else torch.empty(1, dtype=torch.int32, device=dev)     # the backward pass's
         grad = torch.empty_like(logits) if want_grad else None
         ws = _workspace(lib.mdnvae_gate_balance_workspace_bytes(T, E), dev)
         call("mdnvae_gate_balance", lp, vp, T, E, int(top_k), dtype, None if ws is None else ws.data_ptr(),
-             0 if ws is None else ws.numel(), loss.data_ptr(), counts.data_ptr(), mean_probs.data_ptr(), n_valid.data_ptr(),
+             0 if ws is None else ws.numel(), loss.data_ptr(), counts.data_ptr(), mean_probs.data_ptr(), None if n_valid is None else n_valid.data_ptr(),
              None if grad is None else grad.data_ptr(), stream())
     return loss, counts, mean_probs, n_valid, grad
 
@@ -2122,7 +2133,7 @@ class _GateBalance(torch.autograd.Function):
         if g_loss is None and g_mean is None:
             return None, None, None
         T, E = logits.shape
-        with torch.cuda.device(logits.device):
+        with _on(logits.device):
             if g_loss is None:
                 g_loss = torch.zeros((), dtype=torch.float32, device=logits.device)
             g_loss, g_mean = _c(g_loss), None if g_mean is None else _c(g_mean)
