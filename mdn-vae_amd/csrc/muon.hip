@@ -23,6 +23,7 @@
 #include <climits>
 #include <cmath>
 #include <cstdlib>
+#include <type_traits>
 #include "common.h"
 #include "../../include/mdnvae_hip.h"
 
@@ -49,6 +50,7 @@ struct MuGeo {
     long off;
     int m, n, mp, np;                    // m <= n, and padded to the tile
     int trans;                           // the caller's matrix is [n][m]
+    int tile;                            // of X X^T (m and n are padded to it)
     int splits, kper;                    // of the k steps of X X^T
     int count;
 };
@@ -67,13 +69,8 @@ struct MuPtrs {
 };
 
 __host__ __device__ inline long mu_tri(int t) { return (long)t * (t + 1) / 2; }
-template <int TILE>
-__host__ __device__ inline long mu_partial_bytes(const MuGeo& g) {
-    return g.splits > 1 ? (long)g.splits * mu_tri(g.mp / TILE) * TILE * TILE * 4 : 0;
-}
-template <int TILE>
 __host__ __device__ inline long mu_matrix_bytes(const MuGeo& g) {
-    return 8L * g.mp * g.np + 8L * g.mp * g.mp + mu_partial_bytes<TILE>(g);
+    return 8L * g.mp * g.np + 8L * g.mp * g.mp + (g.splits > 1 ? (long)g.splits * mu_tri(g.mp / g.tile) * g.tile * g.tile * 4 : 0);
 }
 
 // entry of workgroup tl: all starts come in with a few wide scalar loads
@@ -166,8 +163,7 @@ __device__ __forceinline__ int mu_at(int row, int half) { return row * 32 + ((ha
 // caller's contiguous dimension ----------------------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(256) void mu_split_kernel(MuTab tab, MuStarts norm, MuPtrs ptrs, MuMom mm, float eps, float scale,
-                                                       const double* __restrict__ partial,
-                                                       char* __restrict__ ws, int tile128) {
+                                                       const double* __restrict__ partial, char* __restrict__ ws) {
     __shared__ float tile[32][65];
     __shared__ double red[4];
     const int e = mu_entry(tab, blockIdx.x);
@@ -209,8 +205,7 @@ __global__ __launch_bounds__(256) void mu_split_kernel(MuTab tab, MuStarts norm,
         hi[k] = h;
         lo[k] = l;
     }
-    const long mb = tile128 ? mu_matrix_bytes<128>(ge) : mu_matrix_bytes<64>(ge);
-    char* dst = ws + ge.off + mat * mb + ((long)(r0 >> 5) * (ge.np >> 4) + (c0 >> 4) + (c8 >> 1)) * MU_STEP + mu_at(r, c8 & 1);
+    char* dst = ws + ge.off + mat * mu_matrix_bytes(ge) + ((long)(r0 >> 5) * (ge.np >> 4) + (c0 >> 4) + (c8 >> 1)) * MU_STEP + mu_at(r, c8 & 1);
     *reinterpret_cast<mu_h8*>(dst) = hi;
     *reinterpret_cast<mu_h8*>(dst + MU_FRAG) = lo;
 }
@@ -278,14 +273,8 @@ __device__ __forceinline__ void mu_tr_block(const char* p, mu_h8 (&out)[N]) {
     for (int i = 0; i < N; ++i) out[i] = mu_join(a[2 * i], a[2 * i + 1]);
 }
 
-#ifndef MU_RING128
-#define MU_RING128 5
-#endif
-#ifndef MU_RING64
-#define MU_RING64 5
-#endif
-template <int TILE>
-__host__ __device__ constexpr int mu_ring() { return TILE == 128 ? MU_RING128 : MU_RING64; }
+// stages of the ring: two workgroups of 128 x 128 fill a CU's 160 KB; four to nine measured alike
+constexpr int MU_RING = 5;
 
 // acc += operand rows [TILE] x operand columns [TILE] over k steps [k0, k1).  Four waves (2 x 2), wave tile TILE/2 squared.
 // Ring of NBUF stages, one k step each, filled by LDS-DMA; one counted wait and one barrier per step.  The operands of
@@ -293,9 +282,12 @@ __host__ __device__ constexpr int mu_ring() { return TILE == 128 ? MU_RING128 : 
 // DMAs are dealt out between the matrix instructions: a wave issues in order, and sixteen DMAs of a step take the
 // CU's address unit 256 clk - issued in one go ahead of the products they cost that time in every step.
 // TR: the row operand is X read down its columns (rsrc: tile (0, first n step), nsteps: n steps of a row of tiles).
-template <int TILE, int TERMS, bool TR, int NBUF>
+// early(): EXTRA loads into registers that the epilogue wants, issued eight steps before the end and not behind it (B X at
+// 4624 x 4624 590 -> 576 us).
+template <int TILE, int TERMS, bool TR, int EXTRA, typename EARLY>
 __device__ __forceinline__ void mu_mainloop(const char* rsrc, const char* csrc, int nsteps, int KS, int k0, int k1, char* smem,
-                                            mu_acc (&acc)[TILE / 64][TILE / 64]) {
+                                            mu_acc (&acc)[TILE / 64][TILE / 64], EARLY early) {
+    constexpr int NBUF = MU_RING;
     constexpr int F = TILE / 32, W = TILE / 64;          // tiles per side, of the workgroup and of a wave
     constexpr int NP = TERMS == 3 ? 2 : 1;
     constexpr int SIDE = F * NP, PPW = 2 * SIDE / 4;     // pieces of one side, pieces per wave
@@ -332,8 +324,7 @@ __device__ __forceinline__ void mu_mainloop(const char* rsrc, const char* csrc, 
         const int pr = TERMS == 3 && t == 0 ? 1 : 0, pc = TERMS == 3 && t == 1 ? 1 : 0;
         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(r[set][i * NP + pr], c[set][j * NP + pc], acc[i][j], 0, 0, 0);
     };
-    const int nk = k1 - k0;
-    if (nk <= 0) return;
+    const int nk = k1 - k0;                              // at least one
     // past the end the last step is fetched again, into a buffer nobody reads any more: every wave always has the same
     // number of operations in flight, and one counted wait fits every iteration
 #pragma unroll
@@ -346,10 +337,10 @@ __device__ __forceinline__ void mu_mainloop(const char* rsrc, const char* csrc, 
     if constexpr (TR) mu_tr_block(my_r, r[0]);
     int b_read = 1, b_fill = NBUF - 1;
     // step `it`: its operands are in (or on their way to) register set `set`
-    auto step = [&](int set, int it) {
+    auto step = [&](int set, int it, auto extra) {
         // own pieces of step it + 1 have landed, own reads of step it are done: after the barrier everybody's, and the buffer
         // of step it - 1 (read before the previous barrier) is free
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NBUF - 3) * PPW) : "memory");
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NBUF - 3) * PPW + decltype(extra)::value) : "memory");
         const int fill = k0 + min(it + NBUF - 1, nk - 1);
         constexpr int HALF = MF * 2 / 3 > 0 ? MF * 2 / 3 : 1;      // reads go first: they have to be back by the next step
 #pragma unroll
@@ -370,10 +361,30 @@ __device__ __forceinline__ void mu_mainloop(const char* rsrc, const char* csrc, 
         b_fill = b_fill + 1 == NBUF ? 0 : b_fill + 1;
         b_read = b_read + 1 == NBUF ? 0 : b_read + 1;
     };
+    std::integral_constant<int, 0> none;
     int it = 0;
+    if constexpr (EXTRA > 0) {
+        static_assert((NBUF - 3) * PPW + EXTRA < 64, "the counter of loads in flight has six bits");
+        static_assert(NBUF == 5, "three steps wait for stages older than the extra loads");
+        std::integral_constant<int, EXTRA> more;
+        if (nk >= 8) {
+            for (; it + 8 < nk; it += 2) {
+                step(0, it, none);
+                step(1, it + 1, none);
+            }
+            early();
+            step(0, it, more);
+            step(1, it + 1, more);
+            step(0, it + 2, more);
+            step(1, it + 3, none);
+            it += 4;
+        } else {
+            early();
+        }
+    }
     for (; it + 1 < nk; it += 2) {
-        step(0, it);
-        step(1, it + 1);
+        step(0, it, none);
+        step(1, it + 1, none);
     }
     if (it < nk) {
 #pragma unroll
@@ -464,27 +475,6 @@ __device__ __forceinline__ void mu_emit_block(const mu_acc& acc, char* dst, cons
         mu_wave_fence();
     }
 }
-// a tile of it (tile row ti of k, tile column tj of rows)
-template <int TILE, int TERMS, bool POLY>
-__device__ __forceinline__ void mu_emit_sym(mu_acc (&acc)[TILE / 64][TILE / 64], char* dst, const char* add, int KS, int ti, int tj,
-                                            const MuScale& sc, char* smem) {
-    constexpr int W = TILE / 64, F = TILE / 32, NP = TERMS == 3 ? 2 : 1;
-    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int rb0 = ti * F + (wid >> 1) * W, cb0 = tj * F + (wid & 1) * W;
-    MuOld old[W][W];
-    if constexpr (POLY) {
-#pragma unroll
-        for (int i = 0; i < W; ++i)
-#pragma unroll
-            for (int j = 0; j < W; ++j) mu_load_block<NP>(old[i][j], add, cb0 + j, KS, (rb0 + i) * 32, threadIdx.x & 63);
-    }
-#pragma unroll
-    for (int i = 0; i < W; ++i)
-#pragma unroll
-        for (int j = 0; j < W; ++j)
-            mu_emit_block<NP, POLY>(acc[i][j], dst, old[i][j], KS, rb0 + i, cb0 + j, ti != tj, sc, smem + wid * 4096);
-}
-
 // tile t of the upper triangle, column by column: (i <= j)
 __device__ __forceinline__ void mu_pair(int t, int& i, int& j) {
     j = (int)((sqrtf(8.0f * (float)t + 1.0f) - 1.0f) * 0.5f);
@@ -526,7 +516,7 @@ __global__ __launch_bounds__(256) void mu_sym_kernel(MuTab tab, int total, char*
     const int s = rest / ntri, t = rest - s * ntri;
     int ti, tj;
     mu_pair_banded(t, T, ti, tj);
-    char* base = ws + ge.off + mat * mu_matrix_bytes<TILE>(ge);
+    char* base = ws + ge.off + mat * mu_matrix_bytes(ge);
     const long xs = 4L * ge.mp * ge.np, as = 4L * ge.mp * ge.mp;
     char* A = base + 2 * xs;
     const int KS = MODE == MU_GRAM ? ge.np >> 4 : ge.mp >> 4;
@@ -540,11 +530,20 @@ __global__ __launch_bounds__(256) void mu_sym_kernel(MuTab tab, int total, char*
 #pragma unroll
             for (int k = 0; k < 16; ++k) acc[i][j][k] = 0.0f;
     const long rows = (long)(TILE / 32) * KS * MU_STEP;
-    mu_mainloop<TILE, TERMS, false, mu_ring<TILE>()>(src + ti * rows, src + tj * rows, 0, KS, MODE == MU_GRAM ? k0 : 0, k1, smem, acc);
+    constexpr int W = TILE / 64, F = TILE / 32, NP = TERMS == 3 ? 2 : 1;
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int rb0 = ti * F + (wid >> 1) * W, cb0 = tj * F + (wid & 1) * W;
+    MuOld old[W][W];                                   // POLY: the tile of A
+    mu_mainloop<TILE, TERMS, false, MODE == MU_POLY ? W * W * 4 * NP : 0>(
+        src + ti * rows, src + tj * rows, 0, KS, MODE == MU_GRAM ? k0 : 0, k1, smem, acc, [&] {
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+#pragma unroll
+                for (int j = 0; j < W; ++j) mu_load_block<NP>(old[i][j], A, cb0 + j, KS, (rb0 + i) * 32, lane);
+        });
     if (MODE == MU_GRAM && splits > 1) {
         // this split's share, as the registers lie (the reducing kernel has the same lanes): 256 bytes per store
         float* part = reinterpret_cast<float*>(A + 2 * as) + ((long)s * ntri + t) * TILE * TILE;
-        const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
 #pragma unroll
         for (int i = 0; i < TILE / 64; ++i)
 #pragma unroll
@@ -556,7 +555,12 @@ __global__ __launch_bounds__(256) void mu_sym_kernel(MuTab tab, int total, char*
                 }
         return;
     }
-    mu_emit_sym<TILE, TERMS, MODE == MU_POLY>(acc, MODE == MU_POLY ? A + as : A, A, ge.mp >> 4, ti, tj, sc, smem);
+    char* dst = MODE == MU_POLY ? A + as : A;
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+            mu_emit_block<NP, MODE == MU_POLY>(acc[i][j], dst, old[i][j], ge.mp >> 4, rb0 + i, cb0 + j, ti != tj, sc, smem + wid * 4096);
 }
 
 // The sum of the splits in fixed order, then what the product kernel does when there is one.  A wave per 32 x 32 block (the
@@ -572,7 +576,7 @@ __global__ __launch_bounds__(256) void mu_reduce_kernel(MuTab tab, char* __restr
     const int local = blockIdx.x / WGS - tab.start[e], mat = local / ntri, t = local - mat * ntri;
     int ti, tj;
     mu_pair_banded(t, T, ti, tj);
-    char* base = ws + ge.off + mat * mu_matrix_bytes<TILE>(ge);
+    char* base = ws + ge.off + mat * mu_matrix_bytes(ge);
     const long xs = 4L * ge.mp * ge.np, as = 4L * ge.mp * ge.mp;
     char* A = base + 2 * xs;
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
@@ -611,7 +615,7 @@ __global__ __launch_bounds__(256) void mu_step_kernel(MuTab tab, int total, MuPt
     // bands of eight tile columns, rows of a band one after the other: 64 neighbours share 8 + 8 operand panels
     const int n0 = rest / (8 * TM) * 8, w = min(8, TN - n0), inband = rest - n0 * TM;
     const int tm = inband / w, tn = n0 + inband - tm * w;
-    char* base = ws + ge.off + mat * mu_matrix_bytes<TILE>(ge);
+    char* base = ws + ge.off + mat * mu_matrix_bytes(ge);
     const long xs = 4L * ge.mp * ge.np, as = 4L * ge.mp * ge.mp;
     const char* X = base + ping * xs;
     char* Y = base + (ping ^ 1) * xs;
@@ -625,18 +629,20 @@ __global__ __launch_bounds__(256) void mu_step_kernel(MuTab tab, int total, MuPt
         for (int j = 0; j < W; ++j)
 #pragma unroll
             for (int k = 0; k < 16; ++k) acc[i][j][k] = 0.0f;
-    mu_mainloop<TILE, TERMS, true, mu_ring<TILE>()>(X + (long)tn * (TILE / 16) * MU_STEP, B + (long)tm * F * KS * MU_STEP, NS, KS, 0, KS, smem, acc);
     const int lane = threadIdx.x & 63;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wid >> 1, wc = wid & 1, h = lane >> 5;
+    MuOld old[W][W];
+    mu_mainloop<TILE, TERMS, true, W * W * 8>(
+        X + (long)tn * (TILE / 16) * MU_STEP, B + (long)tm * F * KS * MU_STEP, NS, KS, 0, KS, smem, acc, [&] {
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+#pragma unroll
+                for (int j = 0; j < W; ++j)
+                    mu_load_block<2>(old[i][j], X, tm * F + wc * W + j, NS, (tn * F + wr * W + i) * 32, lane);
+        });
     const long len = (long)ge.m * ge.n;
     T* out = LAST ? static_cast<T*>(ptrs.p[e]) + mat * len : nullptr;
-    MuOld old[W][W];
-#pragma unroll
-    for (int i = 0; i < W; ++i)
-#pragma unroll
-        for (int j = 0; j < W; ++j)
-            mu_load_block<2>(old[i][j], X, tm * F + wc * W + j, NS, (tn * F + wr * W + i) * 32, lane);
 #pragma unroll
     for (int i = 0; i < W; ++i)
 #pragma unroll
@@ -974,16 +980,8 @@ static bool mu_small(const MuJob& j) {
     return m <= 128 && n <= MU_SMALL_ENTRIES && m * n + m * m <= MU_SMALL_ENTRIES;
 }
 
-#ifndef MU_TW
-#define MU_TW 512
-#endif
-#ifndef MU_TMIN
-#define MU_TMIN 16
-#endif
-constexpr int MU_TARGET_WGS = MU_TW;               // two workgroups per CU: what the splits of X X^T aim at
-#ifndef MU_T128
-#define MU_T128 256
-#endif
+constexpr int MU_CUS = 256;
+constexpr int MU_SPLIT_WGS = 512, MU_SPLIT_STEPS = 32;      // X X^T: workgroups aimed at, fewest k steps of one
 constexpr long MU_PASS_BYTES = 1L << 30;         // workspace beyond which a batch is run in several passes
 constexpr long MU_MAX_SIDE = 65536, MU_MAX_LONG = 1L << 24, MU_MAX_ENTRIES = 1L << 36;
 
@@ -994,20 +992,41 @@ static bool mu_shape_ok(long rows, long cols) {
 
 // The matrices of one pass that take the tiled kernels: at most MU_MAX shapes.
 struct MuPlan {
-    int tile, n;
+    int tile, tile_poly, tile_step, n;
     MuGeo geo[MU_MAX];
     long norm_blocks, bytes;
 };
 
-// 128 x 128 output tiles where there are enough of them for every CU, 64 x 64 where there are not
+// What a launch of products takes, in k steps of a 64 x 64 tile.  A k step of a 128 x 128 tile costs a CU twice one of
+// 64 x 64 (0.33 and 0.16 us: four times the work), but its workgroups go in whole rounds of the 256 CUs where the small ones
+// even out, and start and write-out of a round weigh more.  Measured: A^2 at m = 1024 24 us (128) and 14 (64), B X at
+// 1024 x 4624 48 and 51, at 16 x 512 x 512 22 and 25, at 2 x 1024 x 7569 119 and 144.
+static double mu_cost(double tiles, double ks, int tile) {
+    return tile == 128 ? std::ceil(tiles / MU_CUS) * (2.0 * ks + 20) : std::max(1.0, tiles / MU_CUS) * ks + 15;
+}
+
 static void mu_plan(const MuJob* jobs, int n, MuPlan& pl) {
-    long t128 = 0;
-    for (int i = 0; i < n; ++i) {
-        const long m = std::min(jobs[i].rows, jobs[i].cols), c = std::max(jobs[i].rows, jobs[i].cols);
-        t128 += jobs[i].count * (mu_up(m, 128) / 128) * (mu_up(c, 128) / 128);
+    double c_gram[2] = {0, 0}, c_poly[2] = {0, 0}, c_step[2] = {0, 0};
+    for (int t = 0; t < 2; ++t) {
+        const int tile = t ? 128 : 64;
+        double gk = 0, p = 0, pk = 0, s = 0, sk = 0;             // tiles, and k steps of all of them
+        for (int i = 0; i < n; ++i) {
+            const double m = (double)mu_up(std::min(jobs[i].rows, jobs[i].cols), tile), c = (double)mu_up(std::max(jobs[i].rows, jobs[i].cols), tile);
+            const double count = (double)jobs[i].count, tri = (double)mu_tri((long)m / tile), all = m / tile * (c / tile);
+            gk += count * tri * (c / 16);
+            p += count * tri, pk += count * tri * (m / 16);
+            s += count * all, sk += count * all * (m / 16);
+        }
+        c_gram[t] = gk * (t ? 2.0 : 1.0);                        // split to fit
+        c_poly[t] = mu_cost(p, pk / p, tile);
+        c_step[t] = mu_cost(s, sk / s, tile);
     }
-    const int tile = t128 >= MU_T128 ? 128 : 64;
+    // one padding for all three products; POLY and STEP may take 64 x 64 tiles of matrices padded to 128
+    const int tile = c_gram[1] + MU_CUS * (std::min(c_poly[0], c_poly[1]) + std::min(c_step[0], c_step[1])) <=
+                             c_gram[0] + MU_CUS * (c_poly[0] + c_step[0]) ? 128 : 64;
     pl.tile = tile;
+    pl.tile_poly = tile == 128 && c_poly[1] <= c_poly[0] ? 128 : 64;
+    pl.tile_step = tile == 128 && c_step[1] <= c_step[0] ? 128 : 64;
     pl.n = n;
     long work = 0;
     for (int i = 0; i < n; ++i) {
@@ -1016,12 +1035,14 @@ static void mu_plan(const MuJob* jobs, int n, MuPlan& pl) {
         g.n = (int)std::max(jobs[i].rows, jobs[i].cols);
         g.mp = (int)mu_up(g.m, tile);
         g.np = (int)mu_up(g.n, tile);
+        g.tile = tile;
         g.trans = jobs[i].rows > jobs[i].cols;
         g.count = (int)jobs[i].count;
         work += jobs[i].count * mu_tri(g.mp / tile) * (g.np / 16);
     }
-    // k steps per workgroup of X X^T so that all of them together fill the chip, no fewer than 16
-    const long target = std::max((long)MU_TMIN, (work + MU_TARGET_WGS - 1) / MU_TARGET_WGS);
+    // k steps per workgroup of X X^T: two workgroups per CU, but a share of fewer than 32 steps costs more to write and sum than it
+    // saves (16 x 512 x 512 in halves: 27 us and one launch more, in one piece 17)
+    const long target = std::max((long)MU_SPLIT_STEPS, (work + MU_SPLIT_WGS - 1) / MU_SPLIT_WGS);
     pl.norm_blocks = 0;
     for (int i = 0; i < n; ++i) {
         MuGeo& g = pl.geo[i];
@@ -1034,7 +1055,7 @@ static void mu_plan(const MuJob* jobs, int n, MuPlan& pl) {
     pl.bytes = mu_up(pl.norm_blocks * 8, 1024);
     for (int i = 0; i < n; ++i) {
         pl.geo[i].off = pl.bytes;
-        pl.bytes += jobs[i].count * (tile == 128 ? mu_matrix_bytes<128>(pl.geo[i]) : mu_matrix_bytes<64>(pl.geo[i]));
+        pl.bytes += jobs[i].count * mu_matrix_bytes(pl.geo[i]);
     }
 }
 
@@ -1085,6 +1106,7 @@ static int mu_run_small(const MuJob* jobs, int n, const MuRun& r) {
         g.mp = (int)mu_up(g.m, 32);
         g.np = (int)mu_up(g.n, 32);
         g.trans = jobs[i].rows > jobs[i].cols;
+        g.tile = 32;
         g.splits = g.kper = 1;
         g.count = (int)jobs[i].count;
         tab.start[i] = (int)at;
@@ -1104,7 +1126,39 @@ static int mu_run_small(const MuJob* jobs, int n, const MuRun& r) {
     return 0;
 }
 
-template <typename T, int TERMS, int TILE>
+template <int TILE, int TERMS>
+constexpr size_t mu_lds() {
+    constexpr size_t lds = (size_t)MU_RING * 2 * (TILE / 32) * (TERMS == 3 ? 2 : 1) * MU_FRAG;
+    static_assert(lds <= 160 * 1024 && lds >= 4 * 4224, "the ring fits LDS and holds the epilogues' blocks");
+    return lds;
+}
+static int mu_allow_lds(const void* kernel, size_t lds) {
+    const hipError_t e = lds > 64 * 1024 ? hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) : hipSuccess;
+    MV_REQUIRE(e == hipSuccess, (int)e, "muon: cannot raise the LDS limit: %s", hipGetErrorString(e));
+    return 0;
+}
+static dim3 mu_grid(int n) { return dim3((unsigned)((n + 7) / 8 * 8)); }      // whole rounds of the eight XCDs
+
+template <int TILE, int TERMS, int MODE>
+static int mu_launch_sym(const MuTab& tab, int n, char* ws, int ping, const MuScale& sc, hipStream_t st) {
+    auto kern = mu_sym_kernel<TILE, TERMS, MODE>;
+    constexpr size_t lds = mu_lds<TILE, TERMS>();
+    if (const int rc = mu_allow_lds(reinterpret_cast<const void*>(kern), lds)) return rc;
+    hipLaunchKernelGGL(kern, mu_grid(n), dim3(256), lds, st, tab, n, ws, ping, sc);
+    MV_LAUNCH_CHECK("mu_sym_kernel");
+    return 0;
+}
+template <typename T, int TILE, int TERMS, bool LAST>
+static int mu_launch_step(const MuTab& tab, int n, const MuPtrs& pt, char* ws, int ping, const MuScale& sc, const MuRun& r) {
+    auto kern = mu_step_kernel<T, TILE, TERMS, LAST>;
+    constexpr size_t lds = mu_lds<TILE, TERMS>();
+    if (const int rc = mu_allow_lds(reinterpret_cast<const void*>(kern), lds)) return rc;
+    hipLaunchKernelGGL(kern, mu_grid(n), dim3(256), lds, r.stream, tab, n, pt, ws, ping, sc, r.decay, r.is_step);
+    MV_LAUNCH_CHECK("mu_step_kernel");
+    return 0;
+}
+
+template <typename T, int TERMS>
 static int mu_run_tiled(const MuJob* jobs, const MuPlan& pl, const MuRun& r, char* ws) {
     MuPtrs pt;
     mu_pointers(jobs, pl.n, pt);
@@ -1113,52 +1167,45 @@ static int mu_run_tiled(const MuJob* jobs, const MuPlan& pl, const MuRun& r, cha
     for (int i = 0; i < MU_MAX; ++i) tab.e[i] = pl.geo[i < pl.n ? i : 0];
     MuStarts norm;
     const int n_norm = mu_starts(pl, norm.s, [](const MuGeo& g) { return ((long)g.m * g.n + MU_NORM_BLOCK - 1) / MU_NORM_BLOCK; });
-    MuTab tsplit = tab, tgram = tab, tpoly = tab, tstep = tab;
+    MuTab tnorm = tab, tsplit = tab, tgram = tab, treduce = tab, tpoly = tab, tstep = tab;
+    for (int i = 0; i <= MU_MAX; ++i) tnorm.start[i] = norm.s[i];
     const int n_split = mu_starts(pl, tsplit.start, [](const MuGeo& g) { return (long)(g.mp / 32) * (g.np / 64); });
-    const int n_gram = mu_starts(pl, tgram.start, [](const MuGeo& g) { return mu_tri(g.mp / TILE) * g.splits; });
-    const int n_poly = mu_starts(pl, tpoly.start, [](const MuGeo& g) { return mu_tri(g.mp / TILE); });
-    const int n_step = mu_starts(pl, tstep.start, [](const MuGeo& g) { return (long)(g.mp / TILE) * (g.np / TILE); });
-    MV_REQUIRE(n_norm && n_split && n_gram && n_poly && n_step, E_SHAPE, "mdnvae_orthogonalize: too many tiles for one launch");
+    const int n_gram = mu_starts(pl, tgram.start, [](const MuGeo& g) { return mu_tri(g.mp / g.tile) * g.splits; });
+    const int n_reduce = mu_starts(pl, treduce.start, [](const MuGeo& g) { return mu_tri(g.mp / g.tile); });
+    const int n_poly = mu_starts(pl, tpoly.start, [&](const MuGeo& g) { return mu_tri(g.mp / pl.tile_poly); });
+    const int n_step = mu_starts(pl, tstep.start, [&](const MuGeo& g) { return (long)(g.mp / pl.tile_step) * (g.np / pl.tile_step); });
+    MV_REQUIRE(n_norm && n_split && n_gram && n_reduce && n_poly && n_step, E_SHAPE, "mdnvae_orthogonalize: too many tiles for one launch");
     bool split = false;
     for (int i = 0; i < pl.n; ++i) split = split || pl.geo[i].splits > 1;
     double* partial = reinterpret_cast<double*>(ws);
-    MuTab tnorm = tab;
-    for (int i = 0; i <= MU_MAX; ++i) tnorm.start[i] = norm.s[i];
     hipLaunchKernelGGL((mu_norm_kernel<T>), dim3(n_norm), dim3(256), 0, r.stream, tnorm, pt, r.mm, partial);
     MV_LAUNCH_CHECK("mu_norm_kernel");
     hipLaunchKernelGGL((mu_split_kernel<T>), dim3(n_split), dim3(256), 0, r.stream, tsplit, norm, pt, r.mm, r.co.eps, r.x0_scale,
-                       (const double*)partial, ws, TILE == 128 ? 1 : 0);
+                       (const double*)partial, ws);
     MV_LAUNCH_CHECK("mu_split_kernel");
-    constexpr size_t lds = (size_t)mu_ring<TILE>() * 2 * (TILE / 32) * (TERMS == 3 ? 2 : 1) * MU_FRAG;
-    static_assert(lds <= 160 * 1024 && lds >= 4 * 4224, "the ring fits LDS and holds the epilogues blocks");
-    const void* kernels[4] = {reinterpret_cast<const void*>(mu_sym_kernel<TILE, TERMS, MU_GRAM>),
-                              reinterpret_cast<const void*>(mu_sym_kernel<TILE, TERMS, MU_POLY>),
-                              reinterpret_cast<const void*>(mu_step_kernel<T, TILE, TERMS, false>),
-                              reinterpret_cast<const void*>(mu_step_kernel<T, TILE, TERMS, true>)};
-    for (const void* k : kernels) {
-        const hipError_t e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-        MV_REQUIRE(e == hipSuccess, (int)e, "mu_sym_kernel: cannot raise the LDS limit: %s", hipGetErrorString(e));
-    }
-    auto grid = [](int n) { return dim3((unsigned)((n + 7) / 8 * 8)); };
     for (int it = 0; it < r.st.steps; ++it) {
         const int ping = it & 1;
-        hipLaunchKernelGGL((mu_sym_kernel<TILE, TERMS, MU_GRAM>), grid(n_gram), dim3(256), lds, r.stream, tgram, n_gram, ws, ping,
-                           r.st.gram[it]);
-        MV_LAUNCH_CHECK("mu_sym_kernel");
+        const bool last = it + 1 == r.st.steps;
+        int rc = pl.tile == 128 ? mu_launch_sym<128, TERMS, MU_GRAM>(tgram, n_gram, ws, ping, r.st.gram[it], r.stream)
+                                : mu_launch_sym<64, TERMS, MU_GRAM>(tgram, n_gram, ws, ping, r.st.gram[it], r.stream);
+        if (rc) return rc;
         if (split) {
-            hipLaunchKernelGGL((mu_reduce_kernel<TILE, TERMS>), dim3(n_poly * (TILE / 64) * (TILE / 64)), dim3(256), 0, r.stream, tpoly, ws, r.st.gram[it]);
+            if (pl.tile == 128)
+                hipLaunchKernelGGL((mu_reduce_kernel<128, TERMS>), dim3(n_reduce * 4), dim3(256), 0, r.stream, treduce, ws, r.st.gram[it]);
+            else
+                hipLaunchKernelGGL((mu_reduce_kernel<64, TERMS>), dim3(n_reduce), dim3(256), 0, r.stream, treduce, ws, r.st.gram[it]);
             MV_LAUNCH_CHECK("mu_reduce_kernel");
         }
-        hipLaunchKernelGGL((mu_sym_kernel<TILE, TERMS, MU_POLY>), grid(n_poly), dim3(256), lds, r.stream, tpoly, n_poly, ws, ping,
-                           r.st.poly[it]);
-        MV_LAUNCH_CHECK("mu_sym_kernel");
-        if (it + 1 < r.st.steps)
-            hipLaunchKernelGGL((mu_step_kernel<T, TILE, TERMS, false>), grid(n_step), dim3(256), lds, r.stream, tstep, n_step, pt, ws,
-                               ping, r.st.step[it], r.decay, r.is_step);
+        rc = pl.tile_poly == 128 ? mu_launch_sym<128, TERMS, MU_POLY>(tpoly, n_poly, ws, ping, r.st.poly[it], r.stream)
+                                 : mu_launch_sym<64, TERMS, MU_POLY>(tpoly, n_poly, ws, ping, r.st.poly[it], r.stream);
+        if (rc) return rc;
+        if (pl.tile_step == 128)
+            rc = last ? mu_launch_step<T, 128, TERMS, true>(tstep, n_step, pt, ws, ping, r.st.step[it], r)
+                      : mu_launch_step<T, 128, TERMS, false>(tstep, n_step, pt, ws, ping, r.st.step[it], r);
         else
-            hipLaunchKernelGGL((mu_step_kernel<T, TILE, TERMS, true>), grid(n_step), dim3(256), lds, r.stream, tstep, n_step, pt, ws,
-                               ping, r.st.step[it], r.decay, r.is_step);
-        MV_LAUNCH_CHECK("mu_step_kernel");
+            rc = last ? mu_launch_step<T, 64, TERMS, true>(tstep, n_step, pt, ws, ping, r.st.step[it], r)
+                      : mu_launch_step<T, 64, TERMS, false>(tstep, n_step, pt, ws, ping, r.st.step[it], r);
+        if (rc) return rc;
     }
     return 0;
 }
@@ -1169,7 +1216,7 @@ static int mu_run(const MuJob* jobs, int n, bool small, const MuRun& r, char* ws
     if (small) return mu_run_small<T>(jobs, n, r);
     MuPlan pl;
     mu_plan(jobs, n, pl);
-    return pl.tile == 128 ? mu_run_tiled<T, TERMS, 128>(jobs, pl, r, ws) : mu_run_tiled<T, TERMS, 64>(jobs, pl, r, ws);
+    return mu_run_tiled<T, TERMS>(jobs, pl, r, ws);
 }
 static int mu_dispatch(const MuJob* jobs, int n, bool small, int dtype, int terms, const MuRun& r, char* ws) {
     if (dtype == MDNVAE_F32)
