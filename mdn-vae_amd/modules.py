@@ -482,6 +482,11 @@ class MDNGateVAE(GCNVAE):
         x = x.reshape(-1, self.n_nodes * self.n_nodes)
         return ops.mdn_outer_loss_terms(nodes, x, gate_logits, self.log_sigma, mu, logvar, self.n_nodes)[0]
 
+    def gate_balance(self, gate_logits, top_k=1, valid=None):
+        """How evenly the gate spreads the subjects over the components: (loss, counts, mean probabilities) of
+        ops.gate_balance_loss, a term to add to `loss` where the gate collapses onto one component."""
+        return ops.gate_balance_loss(gate_logits, top_k, valid)
+
     def expected(self, comp, gate_logits):
         """Mixture mean sum_k pi_k m_k [B, N*N] (a library batched GEMM over the K components)."""
         pi = ops.softmax_rows(gate_logits)

@@ -2073,7 +2073,10 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
         return
     etype, dt, dev, n = _element_type(params[0], "params[0]"), params[0].dtype, params[0].device, len(params)
     rows, cols = (ctypes.c_long * n)(), (ctypes.c_long * n)()
+    tensor = torch.Tensor
     for i, (p, g, m) in enumerate(zip(params, grads, momenta)):
+        if not (isinstance(p, tensor) and isinstance(g, tensor) and isinstance(m, tensor)):
+            _refuse_muon(i, p, g, m, dt, dev)
         shape = p.shape
         if not (p.dtype == dt == g.dtype and m.dtype == torch.float32 and g.shape == shape == m.shape and len(shape) > 1
                 and p.device == dev == g.device and m.device == dev and p.is_contiguous() and g.is_contiguous() and m.is_contiguous()):

@@ -142,11 +142,29 @@ class Trainer:
 
     `fast_wgrad`: the weight-gradient products of the large dense layers keep two bf16 parts per operand
     (ops.arithmetic(wgrad="bf16x3"): about 1e-5 of a gradient's norm, 1e-3 of single entries) instead of the
-    default two fp16 parts (fp32 dot-product level); a few percent faster."""
+    default two fp16 parts (fp32 dot-product level); a few percent faster.
+
+    `optimizer`: "adam" (the reference's) or "muon": weights of two and more dimensions (a convolution's as [out, rest])
+    take orthogonalised momentum updates (ops.muon_step with `muon_lr`, `muon_momentum`, `muon_nesterov`,
+    `muon_weight_decay`), all other parameters Adam with `lr`.  `muon_params(name, parameter) -> bool` chooses otherwise.
+    Gradients of symmetric-input first layers are unfolded for it (`folded_adam` is an Adam layout).
+
+    `gate_balance` (loss_mode "mdn"): adds gate_balance * batch * ops.gate_balance_loss(gate logits, gate_top_k)[0] to the
+    (sum-reduced) loss, which keeps the mixture's gate from handing all subjects to one component; the counts of the last
+    step are in `gate_counts` (on the device).  With data-parallel ranks each rank balances its own shard."""
 
     def __init__(self, model, loss_mode, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, group=None, fused_loss=True,
-                 overlap_floats=1 << 20, direct_grads=True, folded_adam=True, fast_wgrad=False):
+                 overlap_floats=1 << 20, direct_grads=True, folded_adam=True, fast_wgrad=False, optimizer="adam", muon_lr=0.02,
+                 muon_momentum=0.95, muon_nesterov=True, muon_weight_decay=0.0, muon_params=None, gate_balance=0.0, gate_top_k=1):
+        if optimizer not in ("adam", "muon"):
+            raise ValueError(f"optimizer {optimizer!r}: 'adam' or 'muon'")
+        if gate_balance and loss_mode != "mdn":
+            raise ValueError("gate_balance is a term of the mixture's loss (loss_mode 'mdn')")
         self.model, self.loss_mode, self.group = model, loss_mode, group
+        self.optimizer = optimizer
+        self.muon = dict(lr=float(muon_lr), momentum=float(muon_momentum), nesterov=bool(muon_nesterov),
+                         weight_decay=float(muon_weight_decay))
+        self.gate_balance, self.gate_top_k, self.gate_counts = float(gate_balance), int(gate_top_k), None
         self.lr, self.betas, self.eps = lr, betas, eps
         self.wgrad_arithmetic = "bf16x3" if fast_wgrad else None
         self._split_graph = False   # a captured data-parallel step: gradients are exchanged between two graphs
@@ -154,12 +172,21 @@ class Trainer:
         # `folded_adam`: weights of symmetric-input first layers keep their gradient folded onto the
         # upper triangle all the way into Adam (moments in the folded layout, both mirror entries
         # take the step): step() then never writes, zeroes or re-reads their unfolded gradient.
-        provider = getattr(model, "folded_grad_params", None)
+        provider = getattr(model, "folded_grad_params", None) if optimizer == "adam" else None
+        choose = muon_params or (lambda name, p: p.dim() >= 2)
+        muon = {id(p) for name, p in model.named_parameters() if optimizer == "muon" and p.requires_grad and choose(name, p)}
+        if any(p.dim() < 2 for p in model.parameters() if id(p) in muon):
+            raise ValueError("muon_params chose a parameter of fewer than two dimensions")
         self._fold = {id(p): (p, n) for p, n in (provider() if (provider and folded_adam and direct_grads) else [])
                       if p.requires_grad}
         # those weights first, then the other early-reduced matrices: what is left is one range
-        self.buf = FlatBuffers(model, front=(lambda p: id(p) in self._fold or bool(early and p.numel() >= overlap_floats))
-                               if (early or self._fold) else None)
+        if muon:                # orthogonalised weights first: Adam's are one range behind them
+            front = (lambda p: id(p) in muon)
+        elif early or self._fold:
+            front = (lambda p: id(p) in self._fold or bool(early and p.numel() >= overlap_floats))
+        else:
+            front = None
+        self.buf = FlatBuffers(model, front=front)
         if self._fold:
             head = self.buf.params[:len(self._fold)]
             if not all(id(p) in self._fold for p in head):       # keep them a prefix of the buffers
@@ -175,6 +202,11 @@ class Trainer:
             shape = (n * (n + 1) // 2, p.shape[0])
             self._fold_m[key] = torch.zeros(shape, dtype=torch.float32, device=p.device)
             self._fold_v[key] = torch.zeros(shape, dtype=torch.float32, device=p.device)
+        self._muon_end = self.buf.offsets[len(muon)]
+        self.muon_buf = torch.zeros(self._muon_end, dtype=torch.float32, device=self.buf.flat_p.device)
+        views = [(o, p) for o, p in zip(self.buf.offsets, self.buf.params[:len(muon)])]
+        self._muon_views = [[flat[o:o + p.numel()].view(p.shape) for o, p in views]
+                            for flat in (self.buf.flat_p, self.buf.flat_g, self.muon_buf)]
         self._defer_fold = False    # inside step(): folded gradients are not unfolded into .grad
         self.steps = 0
         self.fused_loss = fused_loss
@@ -278,8 +310,14 @@ class Trainer:
                 nodes.detach(), target.reshape(target.shape[0], -1), gate_logits.detach(), m.log_sigma.detach(),
                 mu.detach(), logvar.detach(), m.n_nodes,
                 symmetric_x=bool(getattr(m, "symmetric_input", False)) and _same_buffer(target, inputs[0]))
+            loss = terms[0]
+            if self.gate_balance:
+                weight = self.gate_balance * gate_logits.shape[0]
+                balance, self.gate_counts, _, g_gate = ops.gate_balance_loss_and_grads(gate_logits.detach(), self.gate_top_k)
+                g_logits = g_logits.add_(g_gate, alpha=weight)
+                loss = torch.add(loss, balance, alpha=weight)
             torch.autograd.backward([nodes, gate_logits, mu, logvar, m.log_sigma], [g_nodes, g_logits, g_mu, g_lv, g_ls])
-            return terms[0]
+            return loss
         if self.fused_loss and self.loss_mode in ops.RECON_MODES and getattr(self.model, "rank_one_sum_decoder", False):
             # plain sum of outer products (the k-NN GCN decoder): loss, KL and gradients from the
             # node vectors, the reconstruction itself is never written
@@ -294,6 +332,9 @@ class Trainer:
         if self.loss_mode == "mdn":
             comp, gate_logits, mu, logvar = out
             loss = self.model.loss(comp, gate_logits, target, mu, logvar)
+            if self.gate_balance:
+                balance, self.gate_counts, _ = ops.gate_balance_loss(gate_logits, self.gate_top_k)
+                loss = loss + (self.gate_balance * gate_logits.shape[0]) * balance
             loss.backward()
             return loss.detach()
         recon, mu, logvar = out[0], out[1], out[2]
@@ -316,7 +357,8 @@ class Trainer:
         self._apply_adam(None)
 
     def _apply_adam(self, dev_state):
-        """Adam over the flat buffers, and over the folded-gradient weights in their own layout.
+        """Adam over the flat buffers, and over the folded-gradient weights in their own layout; with optimizer="muon" the
+        orthogonalised step of the weights in front, and Adam over the rest.
         dev_state = (step counter, coefficient pair) on the device for a captured step, else None."""
         folded = []
         for work, gt, param, n_nodes in self._folded:
@@ -332,7 +374,9 @@ class Trainer:
         if len(folded) != len(self._fold):
             raise RuntimeError("Trainer: a symmetric-input weight received no folded gradient in this step (a backward "
                                "pass outside Trainer.forward_backward?); build the trainer with folded_adam=False")
-        lo = self._fold_end
+        lo = max(self._fold_end, self._muon_end)
+        if self._muon_end:
+            ops.muon_step(*self._muon_views, **self.muon)
         args = (float(self.lr), float(self.betas[0]), float(self.betas[1]), float(self.eps), 1.0, stream())
         rest = (ptr(self.buf.flat_p[lo:]), ptr(self.buf.flat_g[lo:]), ptr(self.exp_avg[lo:]), ptr(self.exp_avg_sq[lo:]),
                 self.buf.numel - lo)
@@ -371,7 +415,7 @@ class Trainer:
         self._g_eps = eps.detach().clone()
         self._g_step = torch.zeros(1, dtype=torch.int32, device=dev)
         self._g_coef = torch.zeros(2, dtype=torch.float32, device=dev)
-        state = [self.buf.flat_p, self.exp_avg, self.exp_avg_sq] + list(self._fold_m.values()) + \
+        state = [self.buf.flat_p, self.exp_avg, self.exp_avg_sq, self.muon_buf] + list(self._fold_m.values()) + \
             list(self._fold_v.values())
         keep = [t.clone() for t in state]
 
