@@ -81,20 +81,14 @@ __device__ __forceinline__ int mu_entry(const MuTab& tab, int tl) {
     return e;
 }
 
-template <typename T>
-__device__ __forceinline__ float mu_load(const T* p) { return (float)*p; }
-
 // u of one entry: with momentum, M <- mu M + g and u = g + mu M (Nesterov) or M; without, g itself
 struct MuMom { float mu; int nesterov; };
 template <typename T>
-__device__ __forceinline__ float mu_update(const T* g, float* mom, long i, const MuMom& mm, bool store) {
+__device__ __forceinline__ float mu_update(const T* g, float* mom, long i, const MuMom& mm) {
     const float gv = (float)g[i];
     if (!mom) return gv;
-    float m = mom[i];
-    if (store) {
-        m = mm.mu * m + gv;
-        mom[i] = m;
-    }
+    const float m = mm.mu * mom[i] + gv;
+    mom[i] = m;
     return mm.nesterov ? gv + mm.mu * m : m;
 }
 
@@ -109,34 +103,55 @@ __global__ __launch_bounds__(256) void mu_norm_kernel(MuTab tab, MuPtrs ptrs, Mu
     const long local = blockIdx.x - tab.start[e], mat = local / per, blk = local - mat * per;
     const T* g = static_cast<const T*>(ptrs.g[e]) + mat * len;
     float* mom = ptrs.mom[e];
-    const long lo = blk * MU_NORM_BLOCK, hi = min(len, lo + MU_NORM_BLOCK);
+    const long lo = blk * MU_NORM_BLOCK;
+    long hi = min(len, lo + MU_NORM_BLOCK);
     double s = 0.0;
     typedef T vec __attribute__((ext_vector_type(4)));
-    if (hi - lo == MU_NORM_BLOCK && ((reinterpret_cast<uintptr_t>(g + lo) & (4 * sizeof(T) - 1)) | (reinterpret_cast<uintptr_t>(mom) & 15)) == 0) {
+    if (((reinterpret_cast<uintptr_t>(g + lo) & (4 * sizeof(T) - 1)) | (reinterpret_cast<uintptr_t>(mom) & 15)) == 0) {
         constexpr int V = MU_NORM_BLOCK / 1024;            // four entries per access, all loads ahead of the stores
-        vec gv[V];
-        mu_f4 mv[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) gv[i] = *reinterpret_cast<const vec*>(g + lo + (i * 256 + threadIdx.x) * 4);
-        if (mom) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) mv[i] = *reinterpret_cast<const mu_f4*>(mom + lo + (i * 256 + threadIdx.x) * 4);
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
+        auto at = [&](int i) { return lo + (i * 256 + threadIdx.x) * 4; };
+        auto take = [&](const vec& gv, const mu_f4& mv, long i) {
             mu_f4 out;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float gk = (float)gv[i][k];
-                out[k] = mom ? mm.mu * mv[i][k] + gk : gk;
+                const float gk = (float)gv[k];
+                out[k] = mom ? mm.mu * mv[k] + gk : gk;
                 const double u = mom && mm.nesterov ? (double)(gk + mm.mu * out[k]) : (double)out[k];
                 s += u * u;
             }
-            if (mom) *reinterpret_cast<mu_f4*>(mom + lo + (i * 256 + threadIdx.x) * 4) = out;
+            if (mom) *reinterpret_cast<mu_f4*>(mom + i) = out;
+        };
+        vec gv[V];
+        mu_f4 mv[V];
+        if (hi - lo == MU_NORM_BLOCK) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) gv[i] = *reinterpret_cast<const vec*>(g + at(i));
+            if (mom) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) mv[i] = *reinterpret_cast<const mu_f4*>(mom + at(i));
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) take(gv[i], mv[i], at(i));
+            hi = lo;                                       // no tail
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (at(i) + 4 <= hi) {
+                    gv[i] = *reinterpret_cast<const vec*>(g + at(i));
+                    if (mom) mv[i] = *reinterpret_cast<const mu_f4*>(mom + at(i));
+                }
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (at(i) + 4 <= hi) take(gv[i], mv[i], at(i));
+        }
+        const long tail = lo + ((hi - lo) & ~3L) + threadIdx.x;
+        if (tail < hi) {
+            const double u = (double)mu_update(g, mom, tail, mm);
+            s += u * u;
         }
     } else {
         for (long i = lo + threadIdx.x; i < hi; i += 256) {
-            const double u = (double)mu_update(g, mom, i, mm, true);
+            const double u = (double)mu_update(g, mom, i, mm);
             s += u * u;
         }
     }
@@ -173,26 +188,29 @@ __global__ __launch_bounds__(256) void mu_split_kernel(MuTab tab, MuStarts norm,
     const int r0 = (t / nt) * 32, c0 = (t % nt) * 64;
     const long len = (long)ge.m * ge.n, nper = (len + MU_NORM_BLOCK - 1) / MU_NORM_BLOCK;
     const double* part = partial + norm.s[e] + mat * nper;
+    const T* g = static_cast<const T*>(ptrs.g[e]) + mat * len;
+    const float* mom = ptrs.mom[e];
+    // this thread's eight entries: along the caller's rows (lanes over columns) or down them; loads first, clamped to entry 0
+    const int tr = ge.trans ? threadIdx.x & 31 : threadIdx.x >> 6, tc = ge.trans ? threadIdx.x >> 5 : threadIdx.x & 63;
+    float gv[8], mv[8];
+    bool ok[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const int r = r0 + tr + (ge.trans ? 0 : 4 * k), c = c0 + tc + (ge.trans ? 8 * k : 0);
+        ok[k] = r < ge.m && c < ge.n;
+        const long at = ok[k] ? (ge.trans ? (long)c * ge.m + r : (long)r * ge.n + c) : 0;
+        gv[k] = (float)g[at];
+        mv[k] = mom ? mom[at] : 0.0f;
+    }
     double s = 0.0;
     for (long i = threadIdx.x; i < nper; i += 256) s += part[i];
     s = wave_sum(s);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-    const T* g = static_cast<const T*>(ptrs.g[e]) + mat * len;
-    float* mom = ptrs.mom[e];
-    if (!ge.trans) {
-        const int c = threadIdx.x & 63;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const int r = (threadIdx.x >> 6) + 4 * k;
-            tile[r][c] = (r0 + r < ge.m && c0 + c < ge.n) ? mu_update(g, mom, (long)(r0 + r) * ge.n + c0 + c, mm, false) : 0.0f;
-        }
-    } else {
-        const int r = threadIdx.x & 31;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const int c = (threadIdx.x >> 5) + 8 * k;
-            tile[r][c] = (r0 + r < ge.m && c0 + c < ge.n) ? mu_update(g, mom, (long)(c0 + c) * ge.m + r0 + r, mm, false) : 0.0f;
-        }
+    for (int k = 0; k < 8; ++k) {
+        // the momentum is this step's already
+        const float u = !mom ? gv[k] : mm.nesterov ? gv[k] + mm.mu * mv[k] : mv[k];
+        tile[tr + (ge.trans ? 0 : 4 * k)][tc + (ge.trans ? 8 * k : 0)] = ok[k] ? u : 0.0f;
     }
     __syncthreads();
     const double inv = mu_inv_norm((red[0] + red[1]) + (red[2] + red[3]), eps, scale);
