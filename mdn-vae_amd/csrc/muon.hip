@@ -159,14 +159,30 @@ __global__ __launch_bounds__(256) void mu_norm_kernel(MuTab tab, MuPtrs ptrs, Mu
     if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
 
-// 1 / max(|u|_F, eps) * scale; a norm that is not finite (an infinity or a NaN in the matrix) gives NaN, and with it a
-// result that is NaN throughout
-__device__ __forceinline__ double mu_inv_norm(double sum, float eps, float scale) {
-    if (!(sum <= 1.7e308)) return __longlong_as_double(0x7ff8000000000000LL);
-    return (double)scale / fmax(sqrt(sum), (double)eps);
-}
+// u scale / max(|u|_F, eps) as ldexp(u, shift) * factor, since the reciprocal alone may lie outside fp32: |u|_F^2 = m 4^e with m
+// in [0.5, 2), shift = -e, factor = scale / sqrt(m).  A norm that is not finite (an infinity or a NaN in the matrix)
+// gives NaN, and with it a result that is NaN throughout.
+struct MuNorm {
+    int shift;
+    float factor;
+    __device__ __forceinline__ MuNorm(double sum, float eps, float scale) {
+        const double least = (double)eps * (double)eps;
+        const double s = sum < least ? least : sum;
+        const int two_e = ((int)((__double_as_longlong(s) >> 52) & 0x7ff) - 1022 + 1) & ~1;      // a normal number: eps is an fp32
+        const float m = (float)ldexp(s, -two_e);
+        shift = -(two_e >> 1);
+        float r = __builtin_amdgcn_rsqf(m);
+        r = r * fmaf(-0.5f * m * r, r, 1.5f);               // one Newton step on the hardware's estimate
+        factor = s <= 1.7e308 ? scale * r : __uint_as_float(0x7fc00000u);
+    }
+    __device__ __forceinline__ float operator()(float u) const { return ldexpf(u, shift) * factor; }
+};
 
+// t = h + l to 22 bits.  t is made a number in a register first: left to itself the compiler rounds the product that t came
+// from straight to fp16 for one use of h and through fp32 for the other, and where the two differ (once in 2^13) h + l is
+// off by an fp16 step - 5e-6 of a tensor's norm.
 __device__ __forceinline__ void mu_parts(float t, _Float16& h, _Float16& l) {
+    asm("" : "+v"(t));
     h = (_Float16)t;
     l = (_Float16)(t - (float)h);
 }
@@ -213,13 +229,13 @@ __global__ __launch_bounds__(256) void mu_split_kernel(MuTab tab, MuStarts norm,
         tile[tr + (ge.trans ? 0 : 4 * k)][tc + (ge.trans ? 8 * k : 0)] = ok[k] ? u : 0.0f;
     }
     __syncthreads();
-    const double inv = mu_inv_norm((red[0] + red[1]) + (red[2] + red[3]), eps, scale);
+    const MuNorm normal((red[0] + red[1]) + (red[2] + red[3]), eps, scale);
     const int r = threadIdx.x >> 3, c8 = threadIdx.x & 7;
     mu_h8 hi, lo;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
         _Float16 h, l;
-        mu_parts((float)((double)tile[r][c8 * 8 + k] * inv), h, l);
+        mu_parts(normal(tile[r][c8 * 8 + k]), h, l);
         hi[k] = h;
         lo[k] = l;
     }
@@ -719,11 +735,14 @@ __global__ __launch_bounds__(256) void mu_step_kernel(MuTab tab, int total, MuPt
 // ---- small matrices: the whole step in one workgroup ----------------------------------------------------------------------
 // X and A in parts fit LDS (mp np + mp mp <= 38912 entries, mp and np multiples of 32): norm, all iterations and the
 // parameter step in one launch, one matrix per workgroup of up to 16 waves.  A 32 x 32 block of a product belongs to one
-// wave; its registers are held until a barrier says that everybody has read what they overwrite.  Always both parts:
-// such a matrix is bound by latencies and barriers, not by its products.
+// wave.  Where two X and both A and B fit (up to 96 x 96) a product goes to the other buffer; else its registers are held until
+// a barrier says that everybody has read what they overwrite.  Always both parts: such a matrix is bound by latencies and
+// barriers, not by its products.
 constexpr int MU_SMALL_ENTRIES = 38912;
 constexpr int MU_SMALL_NT = 1024;
 constexpr int MU_SMALL_BLOCKS = (MU_SMALL_ENTRIES / 1024 + 15) / 16;      // 32 x 32 blocks of X per wave
+
+__host__ __device__ inline bool mu_small_apart(int mp, int np) { return 2 * (mp * np + mp * mp) <= MU_SMALL_ENTRIES; }
 
 struct MuSteps {                                   // per iteration: the three products' scales
     int steps;
@@ -776,8 +795,12 @@ __global__ __launch_bounds__(MU_SMALL_NT) void mu_small_kernel(MuTab tab, MuPtrs
     float* mom = ptrs.mom[e];
     T* out = static_cast<T*>(ptrs.p[e]) + mat * len;
     const int NS = ge.np >> 4, KS = ge.mp >> 4, MB = ge.mp >> 5, NB = ge.np >> 5;
-    char* X = smem;
-    char* A = smem + 4 * ge.mp * ge.np;
+    const int x_bytes = 4 * ge.mp * ge.np, a_bytes = 4 * ge.mp * ge.mp;
+    const bool apart = mu_small_apart(ge.mp, ge.np);
+    char* X = smem;                                         // and, apart, Y, A, B behind it
+    char* Y = apart ? X + x_bytes : X;
+    char* A = Y + x_bytes;
+    char* B = apart ? A + a_bytes : A;
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, nt = blockDim.x, waves = nt >> 6;
     const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const MuLane ln = mu_lane(lane);
@@ -827,7 +850,7 @@ __global__ __launch_bounds__(MU_SMALL_NT) void mu_small_kernel(MuTab tab, MuPtrs
         if (mom && tid == 0) mom[0] = m0;
         s = 0.0;
         for (int i = 0; i < waves; ++i) s += red[i];
-        const double inv = mu_inv_norm(s, eps, x_scale);
+        const MuNorm normal(s, eps, x_scale);
         for (int ch = tid; ch < chunks; ch += nt) {         // the thread's own chunks
             const int r = ch / per_row, c8 = ch - r * per_row;
             char* dst = place(r, c8);
@@ -836,7 +859,7 @@ __global__ __launch_bounds__(MU_SMALL_NT) void mu_small_kernel(MuTab tab, MuPtrs
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 _Float16 a, b;
-                mu_parts((float)((double)(k < 4 ? lo4[k & 3] : hi4[k & 3]) * inv), a, b);
+                mu_parts(normal(k < 4 ? lo4[k & 3] : hi4[k & 3]), a, b);
                 hi[k] = a;
                 lo[k] = b;
             }
@@ -854,30 +877,36 @@ __global__ __launch_bounds__(MU_SMALL_NT) void mu_small_kernel(MuTab tab, MuPtrs
     const bool mine = wid < MB * MB;                        // at most 16 blocks of A: one per wave
     // the two n steps of a block of X are MU_STEP apart here, not 512 bytes
     const int tr_extra = ((lane >> 4) & 1) * (MU_STEP - 512);
+    // the scales of all iterations, one per lane: a memory access less in every phase
+    const int sl = min(lane, st.steps - 1);
+    const float gram_acc = st.gram[sl].f_acc, poly_acc = st.poly[sl].f_acc, poly_add = st.poly[sl].f_add, step_acc = st.step[sl].f_acc,
+                step_add = st.step[sl].f_add;
+    auto at_step = [](float v, int it) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), it)); };
     for (int it = 0; it < st.steps; ++it) {
         // A = X X^T
         mu_acc acc;
         if (mine) {
             mu_small_product<false>(X + rb * NS * MU_STEP, X + cb * NS * MU_STEP, NS, 0, ln, 0, acc);
-            const float f = st.gram[it].f_acc;
+            const float f = at_step(gram_acc, it);
 #pragma unroll
             for (int k = 0; k < 16; ++k) acc[k] *= f;
 #pragma unroll
             for (int q = 0; q < 4; ++q) put(A + mu_block_at(cb, KS, rb * 32, q, lane), acc, q);
         }
         __syncthreads();
-        // B = b A + c A^2, over A
+        // B = b A + c A^2
         if (mine) {
             mu_small_product<false>(A + rb * KS * MU_STEP, A + cb * KS * MU_STEP, KS, 0, ln, 0, acc);
             MuOld old;
             mu_load_block<2>(old, A, cb, KS, rb * 32, lane);
+            const float f = at_step(poly_acc, it), f_add = at_step(poly_add, it);
 #pragma unroll
-            for (int k = 0; k < 16; ++k) acc[k] = acc[k] * st.poly[it].f_acc + mu_old<2>(old, k >> 2, k & 3) * st.poly[it].f_add;
+            for (int k = 0; k < 16; ++k) acc[k] = acc[k] * f + mu_old<2>(old, k >> 2, k & 3) * f_add;
         }
-        __syncthreads();
+        if (!apart) __syncthreads();
         if (mine) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) put(A + mu_block_at(cb, KS, rb * 32, q, lane), acc, q);
+            for (int q = 0; q < 4; ++q) put(B + mu_block_at(cb, KS, rb * 32, q, lane), acc, q);
         }
         __syncthreads();
         // X <- a X + B X
@@ -887,25 +916,25 @@ __global__ __launch_bounds__(MU_SMALL_NT) void mu_small_kernel(MuTab tab, MuPtrs
             const int id = wid + b * waves;
             if (id < MB * NB) {
                 const int nb = id / MB, mb = id - nb * MB;
-                mu_small_product<true>(X + nb * 2 * MU_STEP, A + mb * KS * MU_STEP, KS, (long)NS * MU_STEP, ln, tr_extra, y[b]);
+                mu_small_product<true>(X + nb * 2 * MU_STEP, B + mb * KS * MU_STEP, KS, (long)NS * MU_STEP, ln, tr_extra, y[b]);
             }
             __builtin_amdgcn_sched_barrier(0);              // a block's operands in registers at a time
         }
-        __syncthreads();
+        if (!apart) __syncthreads();
         const bool last = it + 1 == st.steps;
+        const float f = at_step(step_acc, it), f_add = at_step(step_add, it);
 #pragma unroll
         for (int b = 0; b < BL; ++b) {
             const int id = wid + b * waves;
             if (id < MB * NB) {
                 const int nb = id / MB, mb = id - nb * MB;
-                MuOld old;                                  // what the block replaces is where it goes
+                MuOld old;
                 mu_load_block<2>(old, X, mb, NS, nb * 32, lane);
 #pragma unroll
-                for (int k = 0; k < 16; ++k)
-                    y[b][k] = y[b][k] * st.step[it].f_acc + mu_old<2>(old, k >> 2, k & 3) * st.step[it].f_add;
+                for (int k = 0; k < 16; ++k) y[b][k] = y[b][k] * f + mu_old<2>(old, k >> 2, k & 3) * f_add;
                 if (!last) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) put(X + mu_block_at(mb, NS, nb * 32, q, lane), y[b], q);
+                    for (int q = 0; q < 4; ++q) put(Y + mu_block_at(mb, NS, nb * 32, q, lane), y[b], q);
                 } else {
                     const int m = mb * 32 + (lane & 31), n = nb * 32 + 4 * h;
                     const int left = m < m_valid ? n_valid - n : 0;                 // columns from n on that exist
@@ -932,6 +961,9 @@ __global__ __launch_bounds__(MU_SMALL_NT) void mu_small_kernel(MuTab tab, MuPtrs
             __builtin_amdgcn_sched_barrier(0);
         }
         __syncthreads();
+        char* const swap = X;
+        X = Y;
+        Y = swap;
     }
 }
 
@@ -1129,7 +1161,7 @@ static int mu_run_small(const MuJob* jobs, int n, const MuRun& r) {
         g.count = (int)jobs[i].count;
         tab.start[i] = (int)at;
         at += jobs[i].count;
-        most = std::max(most, 4L * g.mp * (g.np + g.mp));
+        most = std::max(most, (mu_small_apart(g.mp, g.np) ? 8L : 4L) * g.mp * (g.np + g.mp));
         blocks = std::max(blocks, (long)(g.mp / 32) * (g.np / 32));
         MV_REQUIRE(at <= (1L << 30), E_SHAPE, "mdnvae_orthogonalize: too many matrices for one launch");
     }
