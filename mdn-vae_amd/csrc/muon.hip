@@ -184,7 +184,7 @@ struct MuNorm {
 __device__ __forceinline__ void mu_parts(float t, _Float16& h, _Float16& l) {
     asm("" : "+v"(t));
     h = (_Float16)t;
-    l = (_Float16)(t - (float)h);
+    l = (_Float16)fmaf((float)h, -1.0f, t);                 // one instruction that takes h as it is
 }
 
 // byte offset of (row, 16-byte half) inside a tile
@@ -318,6 +318,8 @@ constexpr int MU_RING = 5;
 // TR: the row operand is X read down its columns (rsrc: tile (0, first n step), nsteps: n steps of a row of tiles).
 // early(): EXTRA loads into registers that the epilogue wants, issued eight steps before the end and not behind it (B X at
 // 4624 x 4624 590 -> 576 us).
+// The counted waits rely on exactly EXTRA loads: mu_load_block's are eight bytes each, no two of a lane
+// adjacent (half tiles lie 16 bytes apart in an order that depends on the row, parts 1 KiB), so none can be joined.
 template <int TILE, int TERMS, bool TR, int EXTRA, typename EARLY>
 __device__ __forceinline__ void mu_mainloop(const char* rsrc, const char* csrc, int nsteps, int KS, int k0, int k1, char* smem,
                                             mu_acc (&acc)[TILE / 64][TILE / 64], EARLY early) {
@@ -737,7 +739,9 @@ __global__ __launch_bounds__(256) void mu_step_kernel(MuTab tab, int total, MuPt
 // parameter step in one launch, one matrix per workgroup of up to 16 waves.  A 32 x 32 block of a product belongs to one
 // wave.  Where two X and both A and B fit (up to 96 x 96) a product goes to the other buffer; else its registers are held until
 // a barrier says that everybody has read what they overwrite.  Always both parts: such a matrix is bound by latencies and
-// barriers, not by its products.
+// barriers, not by its products (68 x 68, five iterations: 28 us, 3.9 of them per iteration, of which the matrix
+// instructions on the SIMD with three of the nine waves are 2.2).  A wave with one block of X keeps it, and its block of A, in fp32 registers from product to product
+// instead of joining the parts it reads back (31 us).
 constexpr int MU_SMALL_ENTRIES = 38912;
 constexpr int MU_SMALL_NT = 1024;
 constexpr int MU_SMALL_BLOCKS = (MU_SMALL_ENTRIES / 1024 + 15) / 16;      // 32 x 32 blocks of X per wave
@@ -781,9 +785,9 @@ __device__ __forceinline__ void mu_small_product(const char* rows, const char* c
     }
 }
 
-// BL: blocks of X per wave
-template <typename T, int BL>
-__global__ __launch_bounds__(MU_SMALL_NT) void mu_small_kernel(MuTab tab, MuPtrs ptrs, MuMom mm, float eps, float x_scale, MuSteps st,
+// BL: blocks of X per wave, NT: most threads
+template <typename T, int BL, int NT>
+__global__ __launch_bounds__(NT) void mu_small_kernel(MuTab tab, MuPtrs ptrs, MuMom mm, float eps, float x_scale, MuSteps st,
                                                                float decay, int is_step) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     __shared__ double red[MU_SMALL_NT / 64];
@@ -811,7 +815,7 @@ __global__ __launch_bounds__(MU_SMALL_NT) void mu_small_kernel(MuTab tab, MuPtrs
         auto place = [&](int r, int c8) { return X + ((r >> 5) * NS + (c8 >> 1)) * MU_STEP + mu_at(r & 31, c8 & 1); };
         const float m0 = mom ? mm.mu * mom[0] + (float)g[0] : 0.0f;
         double s = 0.0;
-#pragma unroll 2
+#pragma unroll 1
         for (int ch = tid; ch < chunks; ch += nt) {
             const int r = ch / per_row, c8 = ch - r * per_row;
             int at[8];                                      // within the matrix: fits an int
@@ -881,6 +885,15 @@ __global__ __launch_bounds__(MU_SMALL_NT) void mu_small_kernel(MuTab tab, MuPtrs
     const int sl = min(lane, st.steps - 1);
     const float gram_acc = st.gram[sl].f_acc, poly_acc = st.poly[sl].f_acc, poly_add = st.poly[sl].f_add, step_acc = st.step[sl].f_acc,
                 step_add = st.step[sl].f_add;
+    mu_acc x;
+    if constexpr (BL == 1) {
+        if (wid < MB * NB) {
+            MuOld old;
+            mu_load_block<2>(old, X, wid % MB, NS, wid / MB * 32, lane);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) x[k] = mu_old<2>(old, k >> 2, k & 3);
+        }
+    }
     auto at_step = [](float v, int it) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), it)); };
     for (int it = 0; it < st.steps; ++it) {
         // A = X X^T
@@ -896,12 +909,11 @@ __global__ __launch_bounds__(MU_SMALL_NT) void mu_small_kernel(MuTab tab, MuPtrs
         __syncthreads();
         // B = b A + c A^2
         if (mine) {
+            const mu_acc kept = acc;                        // the wave's block of A is still in its registers
             mu_small_product<false>(A + rb * KS * MU_STEP, A + cb * KS * MU_STEP, KS, 0, ln, 0, acc);
-            MuOld old;
-            mu_load_block<2>(old, A, cb, KS, rb * 32, lane);
             const float f = at_step(poly_acc, it), f_add = at_step(poly_add, it);
 #pragma unroll
-            for (int k = 0; k < 16; ++k) acc[k] = acc[k] * f + mu_old<2>(old, k >> 2, k & 3) * f_add;
+            for (int k = 0; k < 16; ++k) acc[k] = acc[k] * f + kept[k] * f_add;
         }
         if (!apart) __syncthreads();
         if (mine) {
@@ -928,10 +940,15 @@ __global__ __launch_bounds__(MU_SMALL_NT) void mu_small_kernel(MuTab tab, MuPtrs
             const int id = wid + b * waves;
             if (id < MB * NB) {
                 const int nb = id / MB, mb = id - nb * MB;
-                MuOld old;
-                mu_load_block<2>(old, X, mb, NS, nb * 32, lane);
+                if constexpr (BL == 1) {                    // one block: the wave still has its X
 #pragma unroll
-                for (int k = 0; k < 16; ++k) y[b][k] = y[b][k] * f + mu_old<2>(old, k >> 2, k & 3) * f_add;
+                    for (int k = 0; k < 16; ++k) y[b][k] = x[k] = y[b][k] * f + x[k] * f_add;
+                } else {
+                    MuOld old;
+                    mu_load_block<2>(old, X, mb, NS, nb * 32, lane);
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) y[b][k] = y[b][k] * f + mu_old<2>(old, k >> 2, k & 3) * f_add;
+                }
                 if (!last) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) put(Y + mu_block_at(mb, NS, nb * 32, q, lane), y[b], q);
@@ -1165,13 +1182,15 @@ static int mu_run_small(const MuJob* jobs, int n, const MuRun& r) {
         blocks = std::max(blocks, (long)(g.mp / 32) * (g.np / 32));
         MV_REQUIRE(at <= (1L << 30), E_SHAPE, "mdnvae_orthogonalize: too many matrices for one launch");
     }
-    // one block of X per wave (up to 128 x 128) keeps everything in registers; with three some wait in scratch memory
-    auto kern = blocks <= MU_SMALL_NT / 64 ? mu_small_kernel<T, 1> : mu_small_kernel<T, MU_SMALL_BLOCKS>;
+    // up to twelve blocks of X (96 x 128) leave a wave half as many registers again (68 x 68: 28 us; 32 with the 128 registers
+    // that sixteen waves have)
+    auto kern = blocks <= 12 ? mu_small_kernel<T, 1, 768>
+                : blocks <= MU_SMALL_NT / 64 ? mu_small_kernel<T, 1, MU_SMALL_NT> : mu_small_kernel<T, MU_SMALL_BLOCKS, MU_SMALL_NT>;
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
                                              4 * MU_SMALL_ENTRIES);
     MV_REQUIRE(e == hipSuccess, (int)e, "mu_small_kernel: cannot raise the LDS limit: %s", hipGetErrorString(e));
-    hipLaunchKernelGGL(kern, dim3((unsigned)at), dim3((unsigned)std::min((long)MU_SMALL_NT, blocks * 64)), (size_t)most, r.stream, tab, pt, r.mm, r.co.eps, r.x0_scale, r.st,
-                       r.decay, r.is_step);
+    hipLaunchKernelGGL(kern, dim3((unsigned)at), dim3((unsigned)std::min((long)MU_SMALL_NT, blocks * 64)), (size_t)most, r.stream, tab, pt,
+                       r.mm, r.co.eps, r.x0_scale, r.st, r.decay, r.is_step);
     MV_LAUNCH_CHECK("mu_small_kernel");
     return 0;
 }
