@@ -1048,7 +1048,7 @@ static bool mu_small(const MuJob& j) {
 }
 
 constexpr int MU_CUS = 256;
-constexpr int MU_SPLIT_WGS = 512, MU_SPLIT_STEPS = 32;      // X X^T: workgroups aimed at, fewest k steps of one
+constexpr int MU_SPLITS[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 32};     // of X X^T that a plan tries
 constexpr long MU_PASS_BYTES = 1L << 30;         // workspace beyond which a batch is run in several passes
 constexpr long MU_MAX_SIDE = 65536, MU_MAX_LONG = 1L << 24, MU_MAX_ENTRIES = 1L << 36;
 
@@ -1064,38 +1064,67 @@ struct MuPlan {
     long norm_blocks, bytes;
 };
 
-// What a launch of products takes, in k steps of a 64 x 64 tile.  A k step of a 128 x 128 tile costs a CU twice one of
-// 64 x 64 (0.33 and 0.16 us: four times the work), but its workgroups go in whole rounds of the 256 CUs where the small ones
-// even out, and start and write-out of a round weigh more.  Measured: A^2 at m = 1024 24 us (128) and 14 (64), B X at
-// 1024 x 4624 48 and 51, at 16 x 512 x 512 22 and 25, at 2 x 1024 x 7569 119 and 144.
-static double mu_cost(double tiles, double ks, int tile) {
-    return tile == 128 ? std::ceil(tiles / MU_CUS) * (2.0 * ks + 20) : std::max(1.0, tiles / MU_CUS) * ks + 15;
+// What a launch of `wgs` workgroups takes (us, without what both tiles share), if the longest of them has `ks` k steps.  One workgroup per
+// CU is bound by its own chain of loads, reads and products; where more share a CU their products add up, and the fullest CU
+// decides.  A 128 x 128 tile is four times the work of 64 x 64 for two to three times the time of a step, but starts and ends
+// more slowly and leaves CUs idle sooner.  The numbers are a fit to products of 160 x 1000 to 4 x 1024 x 2048, each tile and 1 to
+// 12 splits measured.  With 64 and with 128 (five iterations, fp32): 160 x 1000 126 and 140 us, 1000 x 1000 214 and 225,
+// 1024 x 2048 276 and 275, 2000 x 2000 737 and 662.
+static double mu_cost(double wgs, double ks, int tile, int terms) {
+    const double n = wgs / MU_CUS, whole = n > 4 ? n + 0.5 : std::ceil(n);       // from the fifth on they even out
+    if (tile == 64) return terms == 3 ? ks * std::max(0.13, 0.115 * whole) : ks * std::max(0.11, 0.07 * whole);
+    const double full = std::ceil(n);
+    if (terms == 3) return 3.0 + ks * (n <= 1 ? 0.22 + 0.12 * n : 0.30 * full);
+    return 2.4 + ks * (n <= 1 ? 0.13 + 0.07 * n : 0.137 * full);
 }
 
-static void mu_plan(const MuJob* jobs, int n, MuPlan& pl) {
-    double c_gram[2] = {0, 0}, c_poly[2] = {0, 0}, c_step[2] = {0, 0};
-    for (int t = 0; t < 2; ++t) {
-        const int tile = t ? 128 : 64;
-        double gk = 0, p = 0, pk = 0, s = 0, sk = 0;             // tiles, and k steps of all of them
+static void mu_plan(const MuJob* jobs, int n, int terms, MuPlan& pl) {
+    double best = 0.0;
+    long best_per = 0;
+    for (int tile = 64; tile <= 128; tile += 64) {
+        // X X^T: `per` k steps per workgroup at most; a split costs a launch more, and its shares are written and read again
+        double gram = 0.0, square[2], step[2], rows[MU_MAX], ks[MU_MAX], tri[MU_MAX], longest = 0.0, per = 0.0;
         for (int i = 0; i < n; ++i) {
-            const double m = (double)mu_up(std::min(jobs[i].rows, jobs[i].cols), tile), c = (double)mu_up(std::max(jobs[i].rows, jobs[i].cols), tile);
-            const double count = (double)jobs[i].count, tri = (double)mu_tri((long)m / tile), all = m / tile * (c / tile);
-            gk += count * tri * (c / 16);
-            p += count * tri, pk += count * tri * (m / 16);
-            s += count * all, sk += count * all * (m / 16);
+            rows[i] = (double)mu_up(std::min(jobs[i].rows, jobs[i].cols), tile);
+            ks[i] = (double)(mu_up(std::max(jobs[i].rows, jobs[i].cols), tile) / 16);
+            tri[i] = (double)jobs[i].count * (double)mu_tri((int)rows[i] / tile);
+            longest = std::max(longest, ks[i]);
         }
-        c_gram[t] = gk * (t ? 2.0 : 1.0);                        // split to fit
-        c_poly[t] = mu_cost(p, pk / p, tile);
-        c_step[t] = mu_cost(s, sk / s, tile);
+        for (const int splits : MU_SPLITS) {
+            const double target = std::ceil(longest / splits), inverse = 1.0 / target;
+            double work = 0.0, shares = 0.0;
+            for (int i = 0; i < n; ++i) {
+                work += tri[i] * ks[i];
+                if (ks[i] > target) shares += tri[i] * std::ceil(ks[i] * inverse);
+            }
+            const double t = mu_cost(work * inverse, target, tile, terms) + (splits > 1 ? 4.5 + shares * tile * tile * 8 / 6.0e6 : 0.0);
+            if (splits == 1 || t < gram) gram = t, per = target;
+        }
+        // A^2 and B X: 64 x 64 tiles of matrices padded to 128 may be the faster ones
+        for (int k = 0; k < 2; ++k) {
+            const int tk = k ? 128 : 64;
+            double most = 1.0, p = 0.0, q = 0.0;
+            for (int i = 0; i < n; ++i) {
+                const double k_steps = rows[i] / 16, tiles = rows[i] / tk, work = (double)jobs[i].count * tiles * k_steps;
+                most = std::max(most, k_steps);
+                p += work * (tiles + 1) / 2;
+                q += work * (ks[i] * 16 / tk);
+            }
+            square[k] = mu_cost(p / most, most, tk, terms);
+            step[k] = mu_cost(q / most, most, tk, terms);
+        }
+        const int poly128 = tile == 128 && square[1] <= square[0], step128 = tile == 128 && step[1] <= step[0];
+        const double cost = gram + square[poly128] + step[step128];
+        if (tile == 64 || cost < best) {
+            best = cost;
+            best_per = (long)per;
+            pl.tile = tile;
+            pl.tile_poly = poly128 ? 128 : 64;
+            pl.tile_step = step128 ? 128 : 64;
+        }
     }
-    // one padding for all three products; POLY and STEP may take 64 x 64 tiles of matrices padded to 128
-    const int tile = c_gram[1] + MU_CUS * (std::min(c_poly[0], c_poly[1]) + std::min(c_step[0], c_step[1])) <=
-                             c_gram[0] + MU_CUS * (c_poly[0] + c_step[0]) ? 128 : 64;
-    pl.tile = tile;
-    pl.tile_poly = tile == 128 && c_poly[1] <= c_poly[0] ? 128 : 64;
-    pl.tile_step = tile == 128 && c_step[1] <= c_step[0] ? 128 : 64;
+    const int tile = pl.tile;
     pl.n = n;
-    long work = 0;
     for (int i = 0; i < n; ++i) {
         MuGeo& g = pl.geo[i];
         g.m = (int)std::min(jobs[i].rows, jobs[i].cols);
@@ -1105,16 +1134,12 @@ static void mu_plan(const MuJob* jobs, int n, MuPlan& pl) {
         g.tile = tile;
         g.trans = jobs[i].rows > jobs[i].cols;
         g.count = (int)jobs[i].count;
-        work += jobs[i].count * mu_tri(g.mp / tile) * (g.np / 16);
     }
-    // k steps per workgroup of X X^T: two workgroups per CU, but a share of fewer than 32 steps costs more to write and sum than it
-    // saves (16 x 512 x 512 in halves: 27 us and one launch more, in one piece 17)
-    const long target = std::max((long)MU_SPLIT_STEPS, (work + MU_SPLIT_WGS - 1) / MU_SPLIT_WGS);
     pl.norm_blocks = 0;
     for (int i = 0; i < n; ++i) {
         MuGeo& g = pl.geo[i];
         const long ks = g.np / 16;
-        const long s = std::max(1L, (ks + target / 2) / target);
+        const long s = (ks + best_per - 1) / best_per;
         g.kper = (int)((ks + s - 1) / s);
         g.splits = (int)((ks + g.kper - 1) / g.kper);
         pl.norm_blocks += jobs[i].count * (((long)g.m * g.n + MU_NORM_BLOCK - 1) / MU_NORM_BLOCK);
@@ -1284,7 +1309,7 @@ static int mu_run(const MuJob* jobs, int n, bool small, const MuRun& r, char* ws
     if (n == 0) return 0;
     if (small) return mu_run_small<T>(jobs, n, r);
     MuPlan pl;
-    mu_plan(jobs, n, pl);
+    mu_plan(jobs, n, TERMS, pl);
     return mu_run_tiled<T, TERMS>(jobs, pl, r, ws);
 }
 static int mu_dispatch(const MuJob* jobs, int n, bool small, int dtype, int terms, const MuRun& r, char* ws) {
@@ -1294,11 +1319,11 @@ static int mu_dispatch(const MuJob* jobs, int n, bool small, int dtype, int term
 }
 
 // matrices of a batch that go through one pass
-static long mu_batch_per_pass(long batch, long rows, long cols) {
+static long mu_batch_per_pass(long batch, long rows, long cols, int terms) {
     MuJob j = {rows, cols, 1, nullptr, nullptr, nullptr, 0.0f};
-    if (mu_small(j)) return batch;
+    if (batch == 1 || mu_small(j)) return batch;
     MuPlan pl;
-    mu_plan(&j, 1, pl);                           // what one matrix takes alone: more splits than in company, if anything
+    mu_plan(&j, 1, terms, pl);                    // what one matrix takes alone: more splits than in company, if anything
     return std::max(1L, std::min(batch, MU_PASS_BYTES / std::max(1L, pl.bytes)));
 }
 
@@ -1319,16 +1344,18 @@ using namespace mdnvae;
 
 extern "C" size_t mdnvae_orthogonalize_workspace_bytes(long batch, long rows, long cols) {
     if (batch < 1 || !mu_shape_ok(rows, cols)) return 0;
-    const long per = mu_batch_per_pass(batch, rows, cols), rest = batch % per;
-    MuJob j = {rows, cols, per, nullptr, nullptr, nullptr, 0.0f};
+    MuJob j = {rows, cols, batch, nullptr, nullptr, nullptr, 0.0f};
     if (mu_small(j)) return 0;
     MuPlan pl;
-    mu_plan(&j, 1, pl);
-    long bytes = pl.bytes;
-    if (rest) {                                   // the last pass plans for itself
-        j.count = rest;
-        mu_plan(&j, 1, pl);
-        bytes = std::max(bytes, pl.bytes);
+    long bytes = 0;
+    for (int terms = 1; terms <= 3; terms += 2) {
+        const long per = mu_batch_per_pass(batch, rows, cols, terms);
+        for (const long count : {per, batch % per}) {                    // the last pass plans for itself
+            if (!count) continue;
+            j.count = count;
+            mu_plan(&j, 1, terms, pl);
+            bytes = std::max(bytes, pl.bytes);
+        }
     }
     return (size_t)bytes;
 }
@@ -1350,7 +1377,7 @@ extern "C" int mdnvae_orthogonalize(const void* x, void* out, long batch, long r
     r.stream = (hipStream_t)stream;
     r.decay = 0.0f;
     r.is_step = 0;
-    const long per = mu_batch_per_pass(batch, rows, cols), size = dtype == MDNVAE_F32 ? 4 : 2;
+    const long per = mu_batch_per_pass(batch, rows, cols, terms), size = dtype == MDNVAE_F32 ? 4 : 2;
     for (long at = 0; at < batch; at += per) {
         MuJob j = {rows, cols, std::min(per, batch - at), static_cast<char*>(out) + at * rows * cols * size,
                    static_cast<const char*>(x) + at * rows * cols * size, nullptr, 0.0f};
@@ -1423,8 +1450,10 @@ extern "C" size_t mdnvae_muon_workspace_bytes(const long* rows, const long* cols
     mu_groups(rows, cols, count, [&](MuJob* jobs, const int*, int n, bool small) {
         if (!small) {
             MuPlan pl;
-            mu_plan(jobs, n, pl);
-            most = std::max(most, pl.bytes);
+            for (int terms = 1; terms <= 3; terms += 2) {
+                mu_plan(jobs, n, terms, pl);
+                most = std::max(most, pl.bytes);
+            }
         }
         return 0;
     });

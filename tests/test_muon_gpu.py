@@ -53,6 +53,22 @@ def test_orthogonalize_matches_float64(shape, dtype):
     assert off(y, exact(x)) <= TOL[dtype]
 
 
+# what the cost of a launch decides: both tiles for each product, X X^T in one piece, in a few and in many (the shares of
+# (129, 20000) number 32, the last of them shorter), a batch that fills the chip
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(160, 1000), (129, 20000), (700, 5000), (1000, 4624), (1500, 1501), (1990, 2000), (4, 1000, 2048)], ids=str)
+def test_large_matrices(shape, dtype):
+    x = gaussian(*shape, seed=sum(shape), dtype=dtype).to(DEV)
+    y = ops.orthogonalize(x, steps=3)
+    a, b, c = ops.NS_COEFFICIENTS
+    want = x.double()
+    want = want / torch.linalg.vector_norm(want, dim=(-2, -1), keepdim=True)
+    for _ in range(3):
+        s = want @ want.transpose(-1, -2).contiguous()
+        want = a * want + (b * s + c * (s @ s)) @ want
+    assert float((y.double() - want).norm() / want.norm()) <= TOL[dtype]
+
+
 @pytest.mark.parametrize("steps", [1, 2, 3, 9, 16])
 @pytest.mark.parametrize("shape", [(40, 70), (150, 260)], ids=str)
 def test_number_of_steps(shape, steps):
