@@ -706,11 +706,12 @@ int mdnvae_graph_features(const float* mats, long count, int n, int weighted_pat
  * The other optimizer for weight matrices (the reference trains with Adam, function/VAE_CNN_NN.py:204).
  * Newton-Schulz iteration on each matrix G [rows][cols] of a batch, m = min(rows, cols):
  *     X = G / max(|G|_F, eps) (transposed if rows > cols);  `steps` times: A = X X^T, X <- a X + (b A + c A^2) X
- * out = X in G's shape and type.  x, out: [batch][rows][cols], fp32 or bf16 (`dtype`); out may be x.  A matrix that
- * holds a NaN or an infinity gives NaN throughout; a zero matrix gives zeros.  terms = 3: fp32-level products
- * (two fp16 parts per operand), 1: one product of the high parts (about 1e-3 of the result's norm: for 16-bit
- * results).  Coefficients that could take a singular value in [0, 1] past 256 are refused.  Workspace: 256-byte
- * aligned, sized by the query (0 where each matrix fits one workgroup). */
+ * out = X in G's shape and type.  x, out: [batch][rows][cols], fp32 or bf16 (`dtype`); out may be x but not overlap it
+ * otherwise.  A matrix that holds a NaN or an infinity gives NaN throughout; a zero matrix gives zeros.  terms = 3:
+ * fp32-level products (two fp16 parts per operand), 1: one product of the high parts (about 1e-3 of the result's norm:
+ * for 16-bit results); matrices that fit one workgroup always have the former.  Coefficients that could take a singular
+ * value in [0, 1] past 256 are refused.  Workspace: 256-byte aligned, sized by the query (0 where each matrix fits one
+ * workgroup). */
 enum { MDNVAE_F32 = 0, MDNVAE_BF16 = 1 };
 enum { MDNVAE_MUON_MAX_STEPS = 16 };
 size_t mdnvae_orthogonalize_workspace_bytes(long batch, long rows, long cols);

@@ -1370,6 +1370,9 @@ extern "C" int mdnvae_orthogonalize(const void* x, void* out, long batch, long r
     MV_REQUIRE(mu_shape_ok(rows, cols) && batch <= (1L << 30), E_SHAPE, "mdnvae_orthogonalize: %ld x [%ld, %ld] is larger than the kernels index", batch,
                rows, cols);
     MV_REQUIRE(x && out, E_ARG, "mdnvae_orthogonalize: null pointer");
+    const uintptr_t from = reinterpret_cast<uintptr_t>(x), to = reinterpret_cast<uintptr_t>(out);
+    const uintptr_t length = (uintptr_t)batch * (uintptr_t)rows * (uintptr_t)cols * (dtype == MDNVAE_F32 ? 4 : 2);
+    MV_REQUIRE(from == to || from + length <= to || to + length <= from, E_ARG, "mdnvae_orthogonalize: out overlaps x (it may only be x itself)");
     const size_t need = mdnvae_orthogonalize_workspace_bytes(batch, rows, cols);
     MV_REQUIRE(workspace_bytes >= need && (workspace || need == 0), E_ARG, "mdnvae_orthogonalize: workspace of %zu bytes, %zu are needed",
                workspace_bytes, need);

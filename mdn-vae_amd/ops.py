@@ -2012,10 +2012,12 @@ def _on(device):
 def orthogonalize(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, arithmetic=None, out=None):
     """The nearest thing to an orthogonal matrix that `steps` Newton-Schulz steps reach from each matrix of x [..., m, n]
     (fp32 or bf16, contiguous): X = x / max(|x|_F, eps), then X <- a X + (b A + c A^2) X with A = X X^T (of the
-    transposed matrix if m > n).  Same shape and type as x; `out` may be given, and may be x.  Not differentiable.
+    transposed matrix if m > n).  Same shape and type as x; `out` may be given and may be x, but not overlap it otherwise.
+    Not differentiable.
 
     arithmetic: 'f16x2' (default for fp32) products from two fp16 parts per operand, fp32-level; 'f16' (default for
-    bf16) one product of the high parts, about 1e-3 of the result's norm, a third of the work.
+    bf16) one product of the high parts, about 1e-3 of the result's norm, a third of the work.  Matrices that fit one
+    workgroup (the smaller side up to 128, 38912 entries of X and A padded to 32) are bound by latency and always take 'f16x2'.
     A matrix that holds a NaN or an infinity becomes NaN throughout (the others of the batch do not), a zero matrix
     stays zero.  Coefficients with which a singular value of [0, 1] could pass 256 are refused."""
     dtype = _element_type(x, "x")

@@ -375,3 +375,11 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="overlaps"):     # views that share their middle
         ops.muon_step([flat[:24].view(4, 6), flat[20:44].view(4, 6)], [g, g], [m, torch.zeros(4, 6, device=DEV)], lr=0.1)
     assert bool((p == 0).all()) and bool((m == 0).all())
+
+
+def test_out_that_overlaps_x_is_refused():
+    buf = gaussian(3, 150, 150).to(DEV)
+    with pytest.raises(RuntimeError, match="overlaps"):
+        ops.orthogonalize(buf[:2], out=buf[1:])
+    want = ops.orthogonalize(buf[:1])
+    assert torch.equal(ops.orthogonalize(buf[:1], out=buf[1:2]), want)

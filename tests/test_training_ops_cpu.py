@@ -29,6 +29,18 @@ def test_orthogonalize_arguments_need_no_gpu():
         assert ortho(lib, **kw) == 0
 
 
+def test_orthogonalize_refuses_an_output_that_overlaps_its_input():
+    lib = _lib.load()
+    # a batch of two: the first result would land on the second matrix before that is read
+    for x, out in [(4096, 4100), (4096, 4096 + 64), (4100, 4096), (4096, 4096 + 127)]:
+        assert ortho(lib, x=x, out=out, batch=2) < 0
+        assert b"overlaps" in lib.mdnvae_last_error()
+    # apart, and the same memory: the next check's turn
+    for x, out in [(4096, 4096 + 2 * 300 * 300 * 4), (4096, 4096)]:
+        assert ortho(lib, x=x, out=out, batch=2, rows=300, cols=300) < 0
+        assert b"workspace" in lib.mdnvae_last_error()
+
+
 def test_workspace_of_small_matrices_is_none_and_of_batches_bounded():
     lib = _lib.load()
     for rows, cols in [(1, 1), (128, 128), (128, 68), (1184, 32), (64, 512)]:
