@@ -1390,17 +1390,35 @@ extern "C" int mdnvae_orthogonalize(const void* x, void* out, long batch, long r
     return 0;
 }
 
-// The matrices of a step in order, `f(jobs, n, small)` for each group of up to MU_MAX that is launched together; stops at the
-// first result that is not 0.
+// The matrices of a step in order, `f(jobs, index, n, small)` for each group of up to MU_MAX that is launched together; stops at
+// the first result that is not 0.  Matrices that fit one workgroup are a group of their own, unless there are others, one group
+// holds all and the plan for it takes 64 x 64 tiles: then their tiles cost the launches of the others less than a launch of
+// their own (a convolutional encoder's list of 192 x 1728 and smaller ones in bf16 200 -> 177 us).  A 128 x 128 tile is too much for them (the gated mixture's
+// 1077 -> 1095 us).
 template <typename F>
-static int mu_groups(const long* rows, const long* cols, int count, F f) {
+static int mu_groups(const long* rows, const long* cols, int count, int terms, F f) {
+    MuJob every[MU_MAX];
+    int tiled = 0, all = 0;
+    for (int i = 0; i < count; ++i) {
+        if (rows[i] == 0 || cols[i] == 0) continue;
+        const MuJob j = {rows[i], cols[i], 1, nullptr, nullptr, nullptr, 0.0f};
+        tiled += !mu_small(j);
+        if (all < MU_MAX) every[all] = j;
+        ++all;
+    }
+    bool together = false;
+    if (tiled > 0 && tiled < all && all <= MU_MAX) {
+        MuPlan pl;
+        mu_plan(every, all, terms, pl);
+        together = pl.tile == 64;
+    }
     for (int pass = 0; pass < 2; ++pass) {
         MuJob jobs[MU_MAX];
         int index[MU_MAX], n = 0;
         for (int i = 0; i < count; ++i) {
             if (rows[i] == 0 || cols[i] == 0) continue;
             MuJob j = {rows[i], cols[i], 1, nullptr, nullptr, nullptr, 0.0f};
-            if (mu_small(j) != (pass == 1)) continue;
+            if ((!together && mu_small(j)) != (pass == 1)) continue;
             jobs[n] = j;
             index[n++] = i;
             if (n == MU_MAX) {
@@ -1450,16 +1468,15 @@ extern "C" size_t mdnvae_muon_workspace_bytes(const long* rows, const long* cols
     for (int i = 0; i < count; ++i)
         if (rows[i] < 0 || cols[i] < 0 || (rows[i] > 0 && cols[i] > 0 && !mu_shape_ok(rows[i], cols[i]))) return 0;
     long most = 0;
-    mu_groups(rows, cols, count, [&](MuJob* jobs, const int*, int n, bool small) {
-        if (!small) {
-            MuPlan pl;
-            for (int terms = 1; terms <= 3; terms += 2) {
+    for (int terms = 1; terms <= 3; terms += 2)
+        mu_groups(rows, cols, count, terms, [&](MuJob* jobs, const int*, int n, bool small) {
+            if (!small) {
+                MuPlan pl;
                 mu_plan(jobs, n, terms, pl);
                 most = std::max(most, pl.bytes);
             }
-        }
-        return 0;
-    });
+            return 0;
+        });
     return (size_t)most;
 }
 
@@ -1495,7 +1512,7 @@ extern "C" int mdnvae_muon_step(void* const* params, const void* const* grads, f
     r.decay = (float)(1.0 - (double)lr * (double)weight_decay);
     r.mm = {momentum, nesterov};
     r.is_step = 1;
-    return mu_groups(rows, cols, count, [&](MuJob* jobs, const int* index, int n, bool small) {
+    return mu_groups(rows, cols, count, terms, [&](MuJob* jobs, const int* index, int n, bool small) {
         for (int k = 0; k < n; ++k) {
             const int i = index[k];
             const double ro = (double)rows[i], co = (double)cols[i];

@@ -2064,8 +2064,8 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
     params and grads: fp32 or bf16 tensors (one type for all), momenta: fp32 tensors of the same shapes; contiguous, on
     one device.  A tensor of more than two dimensions (a convolution's weight) counts as [first, all the others].
     scale: 'shape' s = sqrt(max(1, rows / cols)), 'rms' s = 0.2 sqrt(max(rows, cols)) (the size of an Adam step), None s = 1.
-    Matrices that fit one workgroup's LDS take one launch together, all the others share each launch of the
-    tiled products.  steps, coefficients, eps, arithmetic: as for `orthogonalize`."""
+    Up to 32 matrices share each launch of the tiled products; those that fit one workgroup's LDS take one launch of
+    their own, or join the others where that is less work.  steps, coefficients, eps, arithmetic: as for `orthogonalize`."""
     params, grads, momenta = list(params), list(grads), list(momenta)
     if not len(params) == len(grads) == len(momenta):
         raise RuntimeError(f"muon_step: {len(params)} parameters, {len(grads)} gradients, {len(momenta)} momenta")
