@@ -1,5 +1,5 @@
 # Builds the gfx950 kernel library in-tree.  `make` (or __graft_entry__.build()) produces
-# mdn-vae_amd/lib/libmdnvae_hip.so; the GPU box only ever loads that prebuilt file.
+# mdn-vae_amd/lib/libmdnvae_hip.so; tests and programs load that file and build nothing.
 HIPCC ?= /opt/rocm/bin/hipcc
 ARCH ?= gfx950
 PKG := mdn-vae_amd
