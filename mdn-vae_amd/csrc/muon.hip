@@ -283,12 +283,13 @@ __device__ __forceinline__ void mu_tr_block(const char* p, mu_h8 (&out)[N]) {
     const unsigned at = (unsigned)(size_t)(__attribute__((address_space(3))) const char*)(p);
     mu_s4 a[2 * N];
     if constexpr (N == 4) {
-        asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:128\n\t"
-                     "ds_read_b64_tr_b16 %2, %8 offset:1024\n\tds_read_b64_tr_b16 %3, %8 offset:1152\n\t"
-                     "ds_read_b64_tr_b16 %4, %8 offset:2048\n\tds_read_b64_tr_b16 %5, %8 offset:2176\n\t"
-                     "ds_read_b64_tr_b16 %6, %8 offset:3072\n\tds_read_b64_tr_b16 %7, %8 offset:3200\n\ts_waitcnt lgkmcnt(0)"
+        asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%9\n\t"
+                     "ds_read_b64_tr_b16 %2, %8 offset:%10\n\tds_read_b64_tr_b16 %3, %8 offset:%11\n\t"
+                     "ds_read_b64_tr_b16 %4, %8 offset:%12\n\tds_read_b64_tr_b16 %5, %8 offset:%13\n\t"
+                     "ds_read_b64_tr_b16 %6, %8 offset:%14\n\tds_read_b64_tr_b16 %7, %8 offset:%15\n\ts_waitcnt lgkmcnt(0)"
                      : "=&v"(a[0]), "=&v"(a[1]), "=&v"(a[2]), "=&v"(a[3]), "=&v"(a[4]), "=&v"(a[5]), "=&v"(a[6]), "=&v"(a[7])
-                     : "v"(at)
+                     : "v"(at), "n"(128), "n"(MU_FRAG), "n"(MU_FRAG + 128), "n"(2 * MU_FRAG), "n"(2 * MU_FRAG + 128), "n"(3 * MU_FRAG),
+                       "n"(3 * MU_FRAG + 128)
                      : "memory");
     } else if constexpr (N == 2) {
         asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:128\n\t"
@@ -740,8 +741,8 @@ __global__ __launch_bounds__(256) void mu_step_kernel(MuTab tab, int total, MuPt
 // wave.  Where two X and both A and B fit (up to 96 x 96) a product goes to the other buffer; else its registers are held until
 // a barrier says that everybody has read what they overwrite.  Always both parts: such a matrix is bound by latencies and
 // barriers, not by its products (68 x 68, five iterations: 28 us, 3.9 of them per iteration, of which the matrix
-// instructions on the SIMD with three of the nine waves are 2.2).  A wave with one block of X keeps it, and its block of A, in fp32 registers from product to product
-// instead of joining the parts it reads back (31 us).
+// instructions on the SIMD with three of the nine waves are 2.2).  A wave with one block of X keeps it, and its block of A, in
+// fp32 registers from product to product instead of joining the parts it reads back (31 us).
 constexpr int MU_SMALL_ENTRIES = 38912;
 constexpr int MU_SMALL_NT = 1024;
 constexpr int MU_SMALL_BLOCKS = (MU_SMALL_ENTRIES / 1024 + 15) / 16;      // 32 x 32 blocks of X per wave
@@ -1367,8 +1368,8 @@ extern "C" int mdnvae_orthogonalize(const void* x, void* out, long batch, long r
     const int bad = mu_check("mdnvae_orthogonalize", dtype, terms, steps, a, b, c, eps, r);
     if (bad) return bad;
     if (batch == 0 || rows == 0 || cols == 0) return 0;
-    MV_REQUIRE(mu_shape_ok(rows, cols) && batch <= (1L << 30), E_SHAPE, "mdnvae_orthogonalize: %ld x [%ld, %ld] is larger than the kernels index", batch,
-               rows, cols);
+    MV_REQUIRE(mu_shape_ok(rows, cols) && batch <= (1L << 30), E_SHAPE,
+               "mdnvae_orthogonalize: %ld x [%ld, %ld] is larger than the kernels index", batch, rows, cols);
     MV_REQUIRE(x && out, E_ARG, "mdnvae_orthogonalize: null pointer");
     const uintptr_t from = reinterpret_cast<uintptr_t>(x), to = reinterpret_cast<uintptr_t>(out);
     const uintptr_t length = (uintptr_t)batch * (uintptr_t)rows * (uintptr_t)cols * (dtype == MDNVAE_F32 ? 4 : 2);
@@ -1393,8 +1394,8 @@ extern "C" int mdnvae_orthogonalize(const void* x, void* out, long batch, long r
 // The matrices of a step in order, `f(jobs, index, n, small)` for each group of up to MU_MAX that is launched together; stops at
 // the first result that is not 0.  Matrices that fit one workgroup are a group of their own, unless there are others, one group
 // holds all and the plan for it takes 64 x 64 tiles: then their tiles cost the launches of the others less than a launch of
-// their own (a convolutional encoder's list of 192 x 1728 and smaller ones in bf16 200 -> 177 us).  A 128 x 128 tile is too much for them (the gated mixture's
-// 1077 -> 1095 us).
+// their own (a convolutional encoder's list of 192 x 1728 and smaller ones in bf16 200 -> 177 us).  A 128 x 128 tile is too much
+// for them (the gated mixture's 1077 -> 1095 us).
 template <typename F>
 static int mu_groups(const long* rows, const long* cols, int count, int terms, F f) {
     MuJob every[MU_MAX];

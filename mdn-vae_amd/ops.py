@@ -2117,8 +2117,8 @@ def _gate_call(logits, top_k, valid, want_grad):
         grad = torch.empty_like(logits) if want_grad else None
         ws = _workspace(lib.mdnvae_gate_balance_workspace_bytes(T, E), dev)
         call("mdnvae_gate_balance", lp, vp, T, E, int(top_k), dtype, None if ws is None else ws.data_ptr(),
-             0 if ws is None else ws.numel(), loss.data_ptr(), counts.data_ptr(), mean_probs.data_ptr(), None if n_valid is None else n_valid.data_ptr(),
-             None if grad is None else grad.data_ptr(), stream())
+             0 if ws is None else ws.numel(), loss.data_ptr(), counts.data_ptr(), mean_probs.data_ptr(),
+             None if n_valid is None else n_valid.data_ptr(), None if grad is None else grad.data_ptr(), stream())
     return loss, counts, mean_probs, n_valid, grad
 
 
