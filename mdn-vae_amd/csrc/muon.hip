@@ -54,18 +54,22 @@ struct MuGeo {
     int splits, kper;                    // of the k steps of X X^T
     int count;
 };
+// Kernel arguments over N entries, 1 or MU_MAX.  A call over one shape has kernels of its own: the table's entry takes two
+// round trips to arguments that are in no cache yet (0.6 us per launch: 16 x 512 x 512 322 -> 302 us, 1024 x 4624 in bf16 288 -> 267).
+template <int N>
 struct MuTab {
-    int n;
-    int start[MU_MAX + 1];               // first workgroup of each entry; INT_MAX past the last
-    MuGeo e[MU_MAX];
+    int start[N + 1];                    // first workgroup of each entry; INT_MAX past the last
+    MuGeo e[N];
 };
-struct MuStarts { int s[MU_MAX + 1]; };
+template <int N>
+struct MuStarts { int s[N + 1]; };
 // p: result or parameter, g: gradient (or the matrix itself), mom: momentum or null; matrix i at + i * stride elements
+template <int N>
 struct MuPtrs {
-    void* p[MU_MAX];
-    const void* g[MU_MAX];
-    float* mom[MU_MAX];
-    float lr_scale[MU_MAX];
+    void* p[N];
+    const void* g[N];
+    float* mom[N];
+    float lr_scale[N];
 };
 
 __host__ __device__ inline long mu_tri(int t) { return (long)t * (t + 1) / 2; }
@@ -74,10 +78,11 @@ __host__ __device__ inline long mu_matrix_bytes(const MuGeo& g) {
 }
 
 // entry of workgroup tl: all starts come in with a few wide scalar loads
-__device__ __forceinline__ int mu_entry(const MuTab& tab, int tl) {
+template <int N>
+__device__ __forceinline__ int mu_entry(const MuTab<N>& tab, int tl) {
     int e = 0;
 #pragma unroll
-    for (int i = 1; i < MU_MAX; ++i) e += tl >= tab.start[i] ? 1 : 0;
+    for (int i = 1; i < N; ++i) e += tl >= tab.start[i] ? 1 : 0;
     return e;
 }
 
@@ -94,13 +99,13 @@ __device__ __forceinline__ float mu_update(const T* g, float* mom, long i, const
 
 // ---- norm pass: momentum, and each workgroup's sum of squares (float64: the squares of finite fp32 numbers neither
 // overflow nor vanish) -------------------------------------------------------------------------------------------------
-template <typename T>
-__global__ __launch_bounds__(256) void mu_norm_kernel(MuTab tab, MuPtrs ptrs, MuMom mm, double* __restrict__ partial) {
+template <int N, typename T>
+__global__ __launch_bounds__(256) void mu_norm_kernel(MuTab<N> tab, MuPtrs<N> ptrs, MuMom mm, double* __restrict__ partial) {
     __shared__ double red[4];
     const int e = mu_entry(tab, blockIdx.x);
     const MuGeo& ge = tab.e[e];
     const long len = (long)ge.m * ge.n, per = (len + MU_NORM_BLOCK - 1) / MU_NORM_BLOCK;
-    const long local = blockIdx.x - tab.start[e], mat = local / per, blk = local - mat * per;
+    const long local = blockIdx.x - (N == 1 ? 0 : tab.start[e]), mat = local / per, blk = local - mat * per;
     const T* g = static_cast<const T*>(ptrs.g[e]) + mat * len;
     float* mom = ptrs.mom[e];
     const long lo = blk * MU_NORM_BLOCK;
@@ -192,18 +197,18 @@ __device__ __forceinline__ int mu_at(int row, int half) { return row * 32 + ((ha
 
 // ---- split pass: X_0 in parts; one workgroup = 32 rows x 64 columns of X, through LDS so that lanes run along the
 // caller's contiguous dimension ----------------------------------------------------------------------------------------
-template <typename T>
-__global__ __launch_bounds__(256) void mu_split_kernel(MuTab tab, MuStarts norm, MuPtrs ptrs, MuMom mm, float eps, float scale,
+template <int N, typename T>
+__global__ __launch_bounds__(256) void mu_split_kernel(MuTab<N> tab, MuStarts<N> norm, MuPtrs<N> ptrs, MuMom mm, float eps, float scale,
                                                        const double* __restrict__ partial, char* __restrict__ ws) {
     __shared__ float tile[32][65];
     __shared__ double red[4];
     const int e = mu_entry(tab, blockIdx.x);
     const MuGeo& ge = tab.e[e];
     const int nt = ge.np / 64, per = (ge.mp / 32) * nt;
-    const int local = blockIdx.x - tab.start[e], mat = local / per, t = local - mat * per;
+    const int local = blockIdx.x - (N == 1 ? 0 : tab.start[e]), mat = local / per, t = local - mat * per;
     const int r0 = (t / nt) * 32, c0 = (t % nt) * 64;
     const long len = (long)ge.m * ge.n, nper = (len + MU_NORM_BLOCK - 1) / MU_NORM_BLOCK;
-    const double* part = partial + norm.s[e] + mat * nper;
+    const double* part = partial + (N == 1 ? 0 : norm.s[e]) + mat * nper;
     const T* g = static_cast<const T*>(ptrs.g[e]) + mat * len;
     const float* mom = ptrs.mom[e];
     // this thread's eight entries: along the caller's rows (lanes over columns) or down them; loads first, clamped to entry 0
@@ -540,8 +545,8 @@ __device__ __forceinline__ int mu_tile_index(int total) {
     return t < total ? t : -1;
 }
 
-template <int TILE, int TERMS, int MODE>
-__global__ __launch_bounds__(256) void mu_sym_kernel(MuTab tab, int total, char* __restrict__ ws, int ping, MuScale sc) {
+template <int N, int TILE, int TERMS, int MODE>
+__global__ __launch_bounds__(256) void mu_sym_kernel(MuTab<N> tab, int total, char* __restrict__ ws, int ping, MuScale sc) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int tl = mu_tile_index(total);
     if (tl < 0) return;
@@ -549,7 +554,7 @@ __global__ __launch_bounds__(256) void mu_sym_kernel(MuTab tab, int total, char*
     const MuGeo& ge = tab.e[e];
     const int T = ge.mp / TILE, ntri = T * (T + 1) / 2;
     const int splits = MODE == MU_GRAM ? ge.splits : 1;
-    const int local = tl - tab.start[e], mat = local / (ntri * splits), rest = local - mat * ntri * splits;
+    const int local = tl - (N == 1 ? 0 : tab.start[e]), mat = local / (ntri * splits), rest = local - mat * ntri * splits;
     const int s = rest / ntri, t = rest - s * ntri;
     int ti, tj;
     mu_pair_banded(t, T, ti, tj);
@@ -602,15 +607,15 @@ __global__ __launch_bounds__(256) void mu_sym_kernel(MuTab tab, int total, char*
 
 // The sum of the splits in fixed order, then what the product kernel does when there is one.  A wave per 32 x 32 block (the
 // blocks of a tile lie one after the other in a share): 16 of them per tile, for there are few tiles where there are splits.
-template <int TILE, int TERMS>
-__global__ __launch_bounds__(256) void mu_reduce_kernel(MuTab tab, char* __restrict__ ws, MuScale sc) {
+template <int N, int TILE, int TERMS>
+__global__ __launch_bounds__(256) void mu_reduce_kernel(MuTab<N> tab, char* __restrict__ ws, MuScale sc) {
     __shared__ __attribute__((aligned(1024))) char smem[4 * 4096];
     constexpr int W = TILE / 64, WGS = W * W;              // workgroups per tile, four blocks each
     const int e = mu_entry(tab, blockIdx.x / WGS);
     const MuGeo& ge = tab.e[e];
     if (ge.splits == 1) return;
     const int T = ge.mp / TILE, ntri = T * (T + 1) / 2;
-    const int local = blockIdx.x / WGS - tab.start[e], mat = local / ntri, t = local - mat * ntri;
+    const int local = blockIdx.x / WGS - (N == 1 ? 0 : tab.start[e]), mat = local / ntri, t = local - mat * ntri;
     int ti, tj;
     mu_pair_banded(t, T, ti, tj);
     char* base = ws + ge.off + mat * mu_matrix_bytes(ge);
@@ -639,8 +644,8 @@ __global__ __launch_bounds__(256) void mu_reduce_kernel(MuTab tab, char* __restr
 
 // STEP: D rows = 128 (64) columns n of X, D columns = rows m, so that a lane's four consecutive rows are consecutive in X's
 // tiles.  LAST: the result leaves in the caller's layout and type.
-template <typename T, int TILE, int TERMS, bool LAST>
-__global__ __launch_bounds__(256) void mu_step_kernel(MuTab tab, int total, MuPtrs ptrs, char* __restrict__ ws, int ping, MuScale sc,
+template <int N, typename T, int TILE, int TERMS, bool LAST>
+__global__ __launch_bounds__(256) void mu_step_kernel(MuTab<N> tab, int total, MuPtrs<N> ptrs, char* __restrict__ ws, int ping, MuScale sc,
                                                       float decay, int is_step) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int tl = mu_tile_index(total);
@@ -648,7 +653,7 @@ __global__ __launch_bounds__(256) void mu_step_kernel(MuTab tab, int total, MuPt
     const int e = mu_entry(tab, tl);
     const MuGeo& ge = tab.e[e];
     const int TM = ge.mp / TILE, TN = ge.np / TILE;
-    const int local = tl - tab.start[e], mat = local / (TM * TN), rest = local - mat * TM * TN;
+    const int local = tl - (N == 1 ? 0 : tab.start[e]), mat = local / (TM * TN), rest = local - mat * TM * TN;
     // bands of eight tile columns, rows of a band one after the other: 64 neighbours share 8 + 8 operand panels
     const int n0 = rest / (8 * TM) * 8, w = min(8, TN - n0), inband = rest - n0 * TM;
     const int tm = inband / w, tn = n0 + inband - tm * w;
@@ -787,15 +792,15 @@ __device__ __forceinline__ void mu_small_product(const char* rows, const char* c
 }
 
 // BL: blocks of X per wave, NT: most threads
-template <typename T, int BL, int NT>
-__global__ __launch_bounds__(NT) void mu_small_kernel(MuTab tab, MuPtrs ptrs, MuMom mm, float eps, float x_scale, MuSteps st,
+template <int N, typename T, int BL, int NT>
+__global__ __launch_bounds__(NT) void mu_small_kernel(MuTab<N> tab, MuPtrs<N> ptrs, MuMom mm, float eps, float x_scale, MuSteps st,
                                                                float decay, int is_step) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     __shared__ double red[MU_SMALL_NT / 64];
     const int e = mu_entry(tab, blockIdx.x);
     const MuGeo& ge = tab.e[e];
     const int m_valid = ge.m, n_valid = ge.n, trans = ge.trans;
-    const long len = (long)m_valid * n_valid, mat = blockIdx.x - tab.start[e];
+    const long len = (long)m_valid * n_valid, mat = blockIdx.x - (N == 1 ? 0 : tab.start[e]);
     const T* g = static_cast<const T*>(ptrs.g[e]) + mat * len;
     float* mom = ptrs.mom[e];
     T* out = static_cast<T*>(ptrs.p[e]) + mat * len;
@@ -1161,8 +1166,9 @@ struct MuRun {                                   // what the launches of a call 
     hipStream_t stream;
 };
 
-static void mu_pointers(const MuJob* jobs, int n, MuPtrs& pt) {
-    for (int i = 0; i < MU_MAX; ++i) {
+template <int N>
+static void mu_pointers(const MuJob* jobs, int n, MuPtrs<N>& pt) {
+    for (int i = 0; i < N; ++i) {
         pt.p[i] = i < n ? jobs[i].p : nullptr;
         pt.g[i] = i < n ? jobs[i].g : nullptr;
         pt.mom[i] = i < n ? jobs[i].mom : nullptr;
@@ -1171,26 +1177,24 @@ static void mu_pointers(const MuJob* jobs, int n, MuPtrs& pt) {
 }
 
 // first workgroup of each entry, and their number (0: more than a grid holds)
-template <typename F>
-static int mu_starts(const MuPlan& pl, int* start, F per_matrix) {
+template <int N, typename F>
+static int mu_starts(const MuPlan& pl, int (&start)[N], F per_matrix) {
     long at = 0;
-    for (int i = 0; i <= MU_MAX; ++i) {
-        start[i] = i <= pl.n ? (int)at : INT_MAX;
+    for (int i = 0; i < N; ++i) {
+        start[i] = i < pl.n ? (int)at : INT_MAX;
         if (i < pl.n) at += pl.geo[i].count * per_matrix(pl.geo[i]);
         if (at > (1L << 30)) return 0;
     }
-    for (int i = pl.n; i <= MU_MAX; ++i) start[i] = INT_MAX;
     return (int)at;
 }
 
-template <typename T>
+template <int N, typename T>
 static int mu_run_small(const MuJob* jobs, int n, const MuRun& r) {
-    MuTab tab;
-    MuPtrs pt;
+    MuTab<N> tab;
+    MuPtrs<N> pt;
     mu_pointers(jobs, n, pt);
-    tab.n = n;
     long at = 0, most = 0, blocks = 4;
-    for (int i = 0; i <= MU_MAX; ++i) tab.start[i] = INT_MAX;
+    for (int i = 0; i <= N; ++i) tab.start[i] = INT_MAX;
     for (int i = 0; i < n; ++i) {
         MuGeo& g = tab.e[i];
         g.off = 0;
@@ -1210,8 +1214,8 @@ static int mu_run_small(const MuJob* jobs, int n, const MuRun& r) {
     }
     // up to twelve blocks of X (96 x 128) leave a wave half as many registers again (68 x 68: 28 us; 32 with the 128 registers
     // that sixteen waves have)
-    auto kern = blocks <= 12 ? mu_small_kernel<T, 1, 768>
-                : blocks <= MU_SMALL_NT / 64 ? mu_small_kernel<T, 1, MU_SMALL_NT> : mu_small_kernel<T, MU_SMALL_BLOCKS, MU_SMALL_NT>;
+    auto kern = blocks <= 12 ? mu_small_kernel<N, T, 1, 768>
+                : blocks <= MU_SMALL_NT / 64 ? mu_small_kernel<N, T, 1, MU_SMALL_NT> : mu_small_kernel<N, T, MU_SMALL_BLOCKS, MU_SMALL_NT>;
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
                                              4 * MU_SMALL_ENTRIES);
     MV_REQUIRE(e == hipSuccess, (int)e, "mu_small_kernel: cannot raise the LDS limit: %s", hipGetErrorString(e));
@@ -1234,18 +1238,18 @@ static int mu_allow_lds(const void* kernel, size_t lds) {
 }
 static dim3 mu_grid(int n) { return dim3((unsigned)((n + 7) / 8 * 8)); }      // whole rounds of the eight XCDs
 
-template <int TILE, int TERMS, int MODE>
-static int mu_launch_sym(const MuTab& tab, int n, char* ws, int ping, const MuScale& sc, hipStream_t st) {
-    auto kern = mu_sym_kernel<TILE, TERMS, MODE>;
+template <int N, int TILE, int TERMS, int MODE>
+static int mu_launch_sym(const MuTab<N>& tab, int n, char* ws, int ping, const MuScale& sc, hipStream_t st) {
+    auto kern = mu_sym_kernel<N, TILE, TERMS, MODE>;
     constexpr size_t lds = mu_lds<TILE, TERMS>();
     if (const int rc = mu_allow_lds(reinterpret_cast<const void*>(kern), lds)) return rc;
     hipLaunchKernelGGL(kern, mu_grid(n), dim3(256), lds, st, tab, n, ws, ping, sc);
     MV_LAUNCH_CHECK("mu_sym_kernel");
     return 0;
 }
-template <typename T, int TILE, int TERMS, bool LAST>
-static int mu_launch_step(const MuTab& tab, int n, const MuPtrs& pt, char* ws, int ping, const MuScale& sc, const MuRun& r) {
-    auto kern = mu_step_kernel<T, TILE, TERMS, LAST>;
+template <int N, typename T, int TILE, int TERMS, bool LAST>
+static int mu_launch_step(const MuTab<N>& tab, int n, const MuPtrs<N>& pt, char* ws, int ping, const MuScale& sc, const MuRun& r) {
+    auto kern = mu_step_kernel<N, T, TILE, TERMS, LAST>;
     constexpr size_t lds = mu_lds<TILE, TERMS>();
     if (const int rc = mu_allow_lds(reinterpret_cast<const void*>(kern), lds)) return rc;
     hipLaunchKernelGGL(kern, mu_grid(n), dim3(256), lds, r.stream, tab, n, pt, ws, ping, sc, r.decay, r.is_step);
@@ -1253,17 +1257,16 @@ static int mu_launch_step(const MuTab& tab, int n, const MuPtrs& pt, char* ws, i
     return 0;
 }
 
-template <typename T, int TERMS>
+template <int N, typename T, int TERMS>
 static int mu_run_tiled(const MuJob* jobs, const MuPlan& pl, const MuRun& r, char* ws) {
-    MuPtrs pt;
+    MuPtrs<N> pt;
     mu_pointers(jobs, pl.n, pt);
-    MuTab tab;
-    tab.n = pl.n;
-    for (int i = 0; i < MU_MAX; ++i) tab.e[i] = pl.geo[i < pl.n ? i : 0];
-    MuStarts norm;
+    MuTab<N> tab;
+    for (int i = 0; i < N; ++i) tab.e[i] = pl.geo[i < pl.n ? i : 0];
+    MuStarts<N> norm;
     const int n_norm = mu_starts(pl, norm.s, [](const MuGeo& g) { return ((long)g.m * g.n + MU_NORM_BLOCK - 1) / MU_NORM_BLOCK; });
-    MuTab tnorm = tab, tsplit = tab, tgram = tab, treduce = tab, tpoly = tab, tstep = tab;
-    for (int i = 0; i <= MU_MAX; ++i) tnorm.start[i] = norm.s[i];
+    MuTab<N> tnorm = tab, tsplit = tab, tgram = tab, treduce = tab, tpoly = tab, tstep = tab;
+    for (int i = 0; i <= N; ++i) tnorm.start[i] = norm.s[i];
     const int n_split = mu_starts(pl, tsplit.start, [](const MuGeo& g) { return (long)(g.mp / 32) * (g.np / 64); });
     const int n_gram = mu_starts(pl, tgram.start, [](const MuGeo& g) { return mu_tri(g.mp / g.tile) * g.splits; });
     const int n_reduce = mu_starts(pl, treduce.start, [](const MuGeo& g) { return mu_tri(g.mp / g.tile); });
@@ -1273,33 +1276,33 @@ static int mu_run_tiled(const MuJob* jobs, const MuPlan& pl, const MuRun& r, cha
     bool split = false;
     for (int i = 0; i < pl.n; ++i) split = split || pl.geo[i].splits > 1;
     double* partial = reinterpret_cast<double*>(ws);
-    hipLaunchKernelGGL((mu_norm_kernel<T>), dim3(n_norm), dim3(256), 0, r.stream, tnorm, pt, r.mm, partial);
+    hipLaunchKernelGGL((mu_norm_kernel<N, T>), dim3(n_norm), dim3(256), 0, r.stream, tnorm, pt, r.mm, partial);
     MV_LAUNCH_CHECK("mu_norm_kernel");
-    hipLaunchKernelGGL((mu_split_kernel<T>), dim3(n_split), dim3(256), 0, r.stream, tsplit, norm, pt, r.mm, r.co.eps, r.x0_scale,
+    hipLaunchKernelGGL((mu_split_kernel<N, T>), dim3(n_split), dim3(256), 0, r.stream, tsplit, norm, pt, r.mm, r.co.eps, r.x0_scale,
                        (const double*)partial, ws);
     MV_LAUNCH_CHECK("mu_split_kernel");
     for (int it = 0; it < r.st.steps; ++it) {
         const int ping = it & 1;
         const bool last = it + 1 == r.st.steps;
-        int rc = pl.tile == 128 ? mu_launch_sym<128, TERMS, MU_GRAM>(tgram, n_gram, ws, ping, r.st.gram[it], r.stream)
-                                : mu_launch_sym<64, TERMS, MU_GRAM>(tgram, n_gram, ws, ping, r.st.gram[it], r.stream);
+        int rc = pl.tile == 128 ? mu_launch_sym<N, 128, TERMS, MU_GRAM>(tgram, n_gram, ws, ping, r.st.gram[it], r.stream)
+                                : mu_launch_sym<N, 64, TERMS, MU_GRAM>(tgram, n_gram, ws, ping, r.st.gram[it], r.stream);
         if (rc) return rc;
         if (split) {
             if (pl.tile == 128)
-                hipLaunchKernelGGL((mu_reduce_kernel<128, TERMS>), dim3(n_reduce * 4), dim3(256), 0, r.stream, treduce, ws, r.st.gram[it]);
+                hipLaunchKernelGGL((mu_reduce_kernel<N, 128, TERMS>), dim3(n_reduce * 4), dim3(256), 0, r.stream, treduce, ws, r.st.gram[it]);
             else
-                hipLaunchKernelGGL((mu_reduce_kernel<64, TERMS>), dim3(n_reduce), dim3(256), 0, r.stream, treduce, ws, r.st.gram[it]);
+                hipLaunchKernelGGL((mu_reduce_kernel<N, 64, TERMS>), dim3(n_reduce), dim3(256), 0, r.stream, treduce, ws, r.st.gram[it]);
             MV_LAUNCH_CHECK("mu_reduce_kernel");
         }
-        rc = pl.tile_poly == 128 ? mu_launch_sym<128, TERMS, MU_POLY>(tpoly, n_poly, ws, ping, r.st.poly[it], r.stream)
-                                 : mu_launch_sym<64, TERMS, MU_POLY>(tpoly, n_poly, ws, ping, r.st.poly[it], r.stream);
+        rc = pl.tile_poly == 128 ? mu_launch_sym<N, 128, TERMS, MU_POLY>(tpoly, n_poly, ws, ping, r.st.poly[it], r.stream)
+                                 : mu_launch_sym<N, 64, TERMS, MU_POLY>(tpoly, n_poly, ws, ping, r.st.poly[it], r.stream);
         if (rc) return rc;
         if (pl.tile_step == 128)
-            rc = last ? mu_launch_step<T, 128, TERMS, true>(tstep, n_step, pt, ws, ping, r.st.step[it], r)
-                      : mu_launch_step<T, 128, TERMS, false>(tstep, n_step, pt, ws, ping, r.st.step[it], r);
+            rc = last ? mu_launch_step<N, T, 128, TERMS, true>(tstep, n_step, pt, ws, ping, r.st.step[it], r)
+                      : mu_launch_step<N, T, 128, TERMS, false>(tstep, n_step, pt, ws, ping, r.st.step[it], r);
         else
-            rc = last ? mu_launch_step<T, 64, TERMS, true>(tstep, n_step, pt, ws, ping, r.st.step[it], r)
-                      : mu_launch_step<T, 64, TERMS, false>(tstep, n_step, pt, ws, ping, r.st.step[it], r);
+            rc = last ? mu_launch_step<N, T, 64, TERMS, true>(tstep, n_step, pt, ws, ping, r.st.step[it], r)
+                      : mu_launch_step<N, T, 64, TERMS, false>(tstep, n_step, pt, ws, ping, r.st.step[it], r);
         if (rc) return rc;
     }
     return 0;
@@ -1308,10 +1311,10 @@ static int mu_run_tiled(const MuJob* jobs, const MuPlan& pl, const MuRun& r, cha
 template <typename T, int TERMS>
 static int mu_run(const MuJob* jobs, int n, bool small, const MuRun& r, char* ws) {
     if (n == 0) return 0;
-    if (small) return mu_run_small<T>(jobs, n, r);
+    if (small) return n == 1 ? mu_run_small<1, T>(jobs, n, r) : mu_run_small<MU_MAX, T>(jobs, n, r);
     MuPlan pl;
     mu_plan(jobs, n, TERMS, pl);
-    return mu_run_tiled<T, TERMS>(jobs, pl, r, ws);
+    return n == 1 ? mu_run_tiled<1, T, TERMS>(jobs, pl, r, ws) : mu_run_tiled<MU_MAX, T, TERMS>(jobs, pl, r, ws);
 }
 static int mu_dispatch(const MuJob* jobs, int n, bool small, int dtype, int terms, const MuRun& r, char* ws) {
     if (dtype == MDNVAE_F32)
