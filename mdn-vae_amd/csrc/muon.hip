@@ -54,8 +54,9 @@ struct MuGeo {
     int splits, kper;                    // of the k steps of X X^T
     int count;
 };
-// Kernel arguments over N entries, 1 or MU_MAX.  A call over one shape has kernels of its own: the table's entry takes two
-// round trips to arguments that are in no cache yet (0.6 us per launch: 16 x 512 x 512 322 -> 302 us, 1024 x 4624 in bf16 288 -> 267).
+// Kernel arguments over N entries, 1 or MU_MAX.  The arguments are in no cache yet when a kernel starts, and a round trip to
+// them is 0.6 us.  So a call over one shape has kernels of its own, without a table to look the entry up in (16 x 512 x 512 322 ->
+// 302 us, 1024 x 4624 in bf16 288 -> 267), and those over a table do so in one round trip (mu_entry).
 template <int N>
 struct MuTab {
     int start[N + 1];                    // first workgroup of each entry; INT_MAX past the last
@@ -77,13 +78,48 @@ __host__ __device__ inline long mu_matrix_bytes(const MuGeo& g) {
     return 8L * g.mp * g.np + 8L * g.mp * g.mp + (g.splits > 1 ? (long)g.splits * mu_tri(g.mp / g.tile) * g.tile * g.tile * 4 : 0);
 }
 
-// entry of workgroup tl: all starts come in with a few wide scalar loads
+// The entry of a workgroup.  Each lane fetches one entry; which is the workgroup's is a ballot over the starts, and its values
+// come from that lane: one round trip to the arguments instead of two, starts and then the entry (a convolutional encoder's
+// list 180 -> 160 us).
+struct MuEntry {
+    MuGeo ge;
+    int e, first;                        // index and first workgroup
+};
+__device__ __forceinline__ int mu_lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ long mu_lane_value(long v, int lane) {
+    const unsigned lo = (unsigned)mu_lane_value((int)v, lane), hi = (unsigned)mu_lane_value((int)(v >> 32), lane);
+    return (long)((unsigned long)hi << 32 | lo);
+}
 template <int N>
-__device__ __forceinline__ int mu_entry(const MuTab<N>& tab, int tl) {
-    int e = 0;
-#pragma unroll
-    for (int i = 1; i < N; ++i) e += tl >= tab.start[i] ? 1 : 0;
-    return e;
+__device__ __forceinline__ MuEntry mu_entry(const MuTab<N>& tab, int tl) {
+    MuEntry o;
+    if constexpr (N == 1) {
+        o.ge = tab.e[0];
+        o.e = o.first = 0;
+    } else {
+        static_assert(N == 32, "lanes 0 to 31");
+        const int l = threadIdx.x & 31, start = tab.start[l];
+        const MuGeo g = tab.e[l];
+        o.e = __popc((unsigned)__ballot(tl >= start)) - 1;
+        o.first = mu_lane_value(start, o.e);
+        o.ge.off = mu_lane_value(g.off, o.e);
+        o.ge.m = mu_lane_value(g.m, o.e);
+        o.ge.n = mu_lane_value(g.n, o.e);
+        o.ge.mp = mu_lane_value(g.mp, o.e);
+        o.ge.np = mu_lane_value(g.np, o.e);
+        o.ge.trans = mu_lane_value(g.trans, o.e);
+        o.ge.tile = mu_lane_value(g.tile, o.e);
+        o.ge.splits = mu_lane_value(g.splits, o.e);
+        o.ge.kper = mu_lane_value(g.kper, o.e);
+        o.ge.count = mu_lane_value(g.count, o.e);
+    }
+    return o;
+}
+// entry e of a pointer array, the same way
+template <int N, typename P>
+__device__ __forceinline__ P* mu_pick(P* const (&a)[N], int e) {
+    if constexpr (N == 1) return a[0];
+    else return reinterpret_cast<P*>(mu_lane_value(reinterpret_cast<long>(a[threadIdx.x & 31]), e));
 }
 
 // u of one entry: with momentum, M <- mu M + g and u = g + mu M (Nesterov) or M; without, g itself
@@ -102,12 +138,13 @@ __device__ __forceinline__ float mu_update(const T* g, float* mom, long i, const
 template <int N, typename T>
 __global__ __launch_bounds__(256) void mu_norm_kernel(MuTab<N> tab, MuPtrs<N> ptrs, MuMom mm, double* __restrict__ partial) {
     __shared__ double red[4];
-    const int e = mu_entry(tab, blockIdx.x);
-    const MuGeo& ge = tab.e[e];
+    const MuEntry entry = mu_entry(tab, blockIdx.x);
+    const MuGeo& ge = entry.ge;
+    const int e = entry.e;
     const long len = (long)ge.m * ge.n, per = (len + MU_NORM_BLOCK - 1) / MU_NORM_BLOCK;
-    const long local = blockIdx.x - (N == 1 ? 0 : tab.start[e]), mat = local / per, blk = local - mat * per;
-    const T* g = static_cast<const T*>(ptrs.g[e]) + mat * len;
-    float* mom = ptrs.mom[e];
+    const long local = blockIdx.x - entry.first, mat = local / per, blk = local - mat * per;
+    const T* g = static_cast<const T*>(mu_pick(ptrs.g, e)) + mat * len;
+    float* mom = mu_pick(ptrs.mom, e);
     const long lo = blk * MU_NORM_BLOCK;
     long hi = min(len, lo + MU_NORM_BLOCK);
     double s = 0.0;
@@ -202,15 +239,16 @@ __global__ __launch_bounds__(256) void mu_split_kernel(MuTab<N> tab, MuStarts<N>
                                                        const double* __restrict__ partial, char* __restrict__ ws) {
     __shared__ float tile[32][65];
     __shared__ double red[4];
-    const int e = mu_entry(tab, blockIdx.x);
-    const MuGeo& ge = tab.e[e];
+    const MuEntry entry = mu_entry(tab, blockIdx.x);
+    const MuGeo& ge = entry.ge;
+    const int e = entry.e;
     const int nt = ge.np / 64, per = (ge.mp / 32) * nt;
-    const int local = blockIdx.x - (N == 1 ? 0 : tab.start[e]), mat = local / per, t = local - mat * per;
+    const int local = blockIdx.x - entry.first, mat = local / per, t = local - mat * per;
     const int r0 = (t / nt) * 32, c0 = (t % nt) * 64;
     const long len = (long)ge.m * ge.n, nper = (len + MU_NORM_BLOCK - 1) / MU_NORM_BLOCK;
     const double* part = partial + (N == 1 ? 0 : norm.s[e]) + mat * nper;
-    const T* g = static_cast<const T*>(ptrs.g[e]) + mat * len;
-    const float* mom = ptrs.mom[e];
+    const T* g = static_cast<const T*>(mu_pick(ptrs.g, e)) + mat * len;
+    const float* mom = mu_pick(ptrs.mom, e);
     // this thread's eight entries: along the caller's rows (lanes over columns) or down them; loads first, clamped to entry 0
     const int tr = ge.trans ? threadIdx.x & 31 : threadIdx.x >> 6, tc = ge.trans ? threadIdx.x >> 5 : threadIdx.x & 63;
     float gv[8], mv[8];
@@ -549,12 +587,12 @@ template <int N, int TILE, int TERMS, int MODE>
 __global__ __launch_bounds__(256) void mu_sym_kernel(MuTab<N> tab, int total, char* __restrict__ ws, int ping, MuScale sc) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int tl = mu_tile_index(total);
+    const MuEntry entry = mu_entry(tab, max(tl, 0));        // ahead of the branch: its loads go with that of `total`
     if (tl < 0) return;
-    const int e = mu_entry(tab, tl);
-    const MuGeo& ge = tab.e[e];
+    const MuGeo& ge = entry.ge;
     const int T = ge.mp / TILE, ntri = T * (T + 1) / 2;
     const int splits = MODE == MU_GRAM ? ge.splits : 1;
-    const int local = tl - (N == 1 ? 0 : tab.start[e]), mat = local / (ntri * splits), rest = local - mat * ntri * splits;
+    const int local = tl - entry.first, mat = local / (ntri * splits), rest = local - mat * ntri * splits;
     const int s = rest / ntri, t = rest - s * ntri;
     int ti, tj;
     mu_pair_banded(t, T, ti, tj);
@@ -611,11 +649,11 @@ template <int N, int TILE, int TERMS>
 __global__ __launch_bounds__(256) void mu_reduce_kernel(MuTab<N> tab, char* __restrict__ ws, MuScale sc) {
     __shared__ __attribute__((aligned(1024))) char smem[4 * 4096];
     constexpr int W = TILE / 64, WGS = W * W;              // workgroups per tile, four blocks each
-    const int e = mu_entry(tab, blockIdx.x / WGS);
-    const MuGeo& ge = tab.e[e];
+    const MuEntry entry = mu_entry(tab, blockIdx.x / WGS);
+    const MuGeo& ge = entry.ge;
     if (ge.splits == 1) return;
     const int T = ge.mp / TILE, ntri = T * (T + 1) / 2;
-    const int local = blockIdx.x / WGS - (N == 1 ? 0 : tab.start[e]), mat = local / ntri, t = local - mat * ntri;
+    const int local = blockIdx.x / WGS - entry.first, mat = local / ntri, t = local - mat * ntri;
     int ti, tj;
     mu_pair_banded(t, T, ti, tj);
     char* base = ws + ge.off + mat * mu_matrix_bytes(ge);
@@ -649,11 +687,12 @@ __global__ __launch_bounds__(256) void mu_step_kernel(MuTab<N> tab, int total, M
                                                       float decay, int is_step) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int tl = mu_tile_index(total);
+    const MuEntry entry = mu_entry(tab, max(tl, 0));        // ahead of the branch: its loads go with that of `total`
     if (tl < 0) return;
-    const int e = mu_entry(tab, tl);
-    const MuGeo& ge = tab.e[e];
+    const MuGeo& ge = entry.ge;
+    const int e = entry.e;
     const int TM = ge.mp / TILE, TN = ge.np / TILE;
-    const int local = tl - (N == 1 ? 0 : tab.start[e]), mat = local / (TM * TN), rest = local - mat * TM * TN;
+    const int local = tl - entry.first, mat = local / (TM * TN), rest = local - mat * TM * TN;
     // bands of eight tile columns, rows of a band one after the other: 64 neighbours share 8 + 8 operand panels
     const int n0 = rest / (8 * TM) * 8, w = min(8, TN - n0), inband = rest - n0 * TM;
     const int tm = inband / w, tn = n0 + inband - tm * w;
@@ -684,7 +723,7 @@ __global__ __launch_bounds__(256) void mu_step_kernel(MuTab<N> tab, int total, M
                     mu_load_block<2>(old[i][j], X, tm * F + wc * W + j, NS, (tn * F + wr * W + i) * 32, lane);
         });
     const long len = (long)ge.m * ge.n;
-    T* out = LAST ? static_cast<T*>(ptrs.p[e]) + mat * len : nullptr;
+    T* out = LAST ? static_cast<T*>(mu_pick(ptrs.p, e)) + mat * len : nullptr;
 #pragma unroll
     for (int i = 0; i < W; ++i)
 #pragma unroll
@@ -797,13 +836,14 @@ __global__ __launch_bounds__(NT) void mu_small_kernel(MuTab<N> tab, MuPtrs<N> pt
                                                                float decay, int is_step) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     __shared__ double red[MU_SMALL_NT / 64];
-    const int e = mu_entry(tab, blockIdx.x);
-    const MuGeo& ge = tab.e[e];
+    const MuEntry entry = mu_entry(tab, blockIdx.x);
+    const MuGeo& ge = entry.ge;
+    const int e = entry.e;
     const int m_valid = ge.m, n_valid = ge.n, trans = ge.trans;
-    const long len = (long)m_valid * n_valid, mat = blockIdx.x - (N == 1 ? 0 : tab.start[e]);
-    const T* g = static_cast<const T*>(ptrs.g[e]) + mat * len;
-    float* mom = ptrs.mom[e];
-    T* out = static_cast<T*>(ptrs.p[e]) + mat * len;
+    const long len = (long)m_valid * n_valid, mat = blockIdx.x - entry.first;
+    const T* g = static_cast<const T*>(mu_pick(ptrs.g, e)) + mat * len;
+    float* mom = mu_pick(ptrs.mom, e);
+    T* out = static_cast<T*>(mu_pick(ptrs.p, e)) + mat * len;
     const int NS = ge.np >> 4, KS = ge.mp >> 4, MB = ge.mp >> 5, NB = ge.np >> 5;
     const int x_bytes = 4 * ge.mp * ge.np, a_bytes = 4 * ge.mp * ge.mp;
     const bool apart = mu_small_apart(ge.mp, ge.np);
