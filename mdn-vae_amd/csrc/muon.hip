@@ -768,7 +768,7 @@ __global__ __launch_bounds__(256) void mu_step_kernel(MuTab<N> tab, int total, M
                 if (is_step) {
                     T p[16];
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) p[k] = ok[k] ? out[at[k]] : (T)0.0f;
+                    for (int k = 0; k < 16; ++k) p[k] = out[ok[k] ? at[k] : 0];      // entry 0 stands in: sixteen 16-bit loads in flight
 #pragma unroll
                     for (int k = 0; k < 16; ++k) v[k] = decay * (float)p[k] - ptrs.lr_scale[e] * v[k];
                 }
