@@ -780,7 +780,7 @@ __global__ __launch_bounds__(256) void mu_step_kernel(MuTab<N> tab, int total, M
 }
 
 // ---- small matrices: the whole step in one workgroup ----------------------------------------------------------------------
-// X and A in parts fit LDS (mp np + mp mp <= 38912 entries, mp and np multiples of 32): norm, all iterations and the
+// X and A in parts fit LDS (mp np + mp mp <= 38912 entries, mp and np multiples of 32; mu_small): norm, all iterations and the
 // parameter step in one launch, one matrix per workgroup of up to 16 waves.  A 32 x 32 block of a product belongs to one
 // wave.  Where two X and both A and B fit (up to 96 x 96) a product goes to the other buffer; else its registers are held until
 // a barrier says that everybody has read what they overwrite.  Always both parts: such a matrix is bound by latencies and
@@ -1088,12 +1088,17 @@ struct MuJob {                                   // one shape: `count` matrices 
 };
 
 static long mu_up(long v, long t) { return (v + t - 1) / t * t; }
+constexpr int MU_CUS = 256;
+
+// Whether each matrix goes to one workgroup: X and A have to fit, and X is a block per wave, or there are matrices for all CUs.  With
+// more blocks one workgroup takes longer over them than the tiled launches do (64 x 544 87 and 78 us, an optimizer step over
+// twenty 133 and 94), but a batch does not (300 of 32 x 1184 209 and 310 us).
 static bool mu_small(const MuJob& j) {
     const long m = mu_up(std::min(j.rows, j.cols), 32), n = mu_up(std::max(j.rows, j.cols), 32);
-    return m <= 128 && n <= MU_SMALL_ENTRIES && m * n + m * m <= MU_SMALL_ENTRIES;
+    return m <= 128 && n <= MU_SMALL_ENTRIES && m * n + m * m <= MU_SMALL_ENTRIES &&
+           (m * n <= 32 * 32 * (MU_SMALL_NT / 64) || j.count >= MU_CUS);
 }
 
-constexpr int MU_CUS = 256;
 constexpr int MU_SPLITS[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 32};     // of X X^T that a plan tries
 constexpr long MU_PASS_BYTES = 1L << 30;         // workspace beyond which a batch is run in several passes
 constexpr long MU_MAX_SIDE = 65536, MU_MAX_LONG = 1L << 24, MU_MAX_ENTRIES = 1L << 36;
@@ -1364,8 +1369,9 @@ static int mu_dispatch(const MuJob* jobs, int n, bool small, int dtype, int term
 
 // matrices of a batch that go through one pass
 static long mu_batch_per_pass(long batch, long rows, long cols, int terms) {
-    MuJob j = {rows, cols, 1, nullptr, nullptr, nullptr, 0.0f};
+    MuJob j = {rows, cols, batch, nullptr, nullptr, nullptr, 0.0f};
     if (batch == 1 || mu_small(j)) return batch;
+    j.count = 1;
     MuPlan pl;
     mu_plan(&j, 1, terms, pl);                    // what one matrix takes alone: more splits than in company, if anything
     return std::max(1L, std::min(batch, MU_PASS_BYTES / std::max(1L, pl.bytes)));

@@ -2016,8 +2016,9 @@ def orthogonalize(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, arithmetic
     Not differentiable.
 
     arithmetic: 'f16x2' (default for fp32) products from two fp16 parts per operand, fp32-level; 'f16' (default for
-    bf16) one product of the high parts, about 1e-3 of the result's norm, a third of the work.  Matrices that fit one
-    workgroup (the smaller side up to 128, 38912 entries of X and A padded to 32) are bound by latency and always take 'f16x2'.
+    bf16) one product of the high parts, about 1e-3 of the result's norm, a third of the work.  Small matrices (up to
+    128 x 128, or 16384 entries padded to 32; somewhat larger ones in batches of hundreds) take one workgroup each, are bound by
+    latency and always have 'f16x2'.
     A matrix that holds a NaN or an infinity becomes NaN throughout (the others of the batch do not), a zero matrix
     stays zero.  Coefficients with which a singular value of [0, 1] could pass 256 are refused."""
     dtype = _element_type(x, "x")
@@ -2064,8 +2065,8 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
     params and grads: fp32 or bf16 tensors (one type for all), momenta: fp32 tensors of the same shapes; contiguous, on
     one device.  A tensor of more than two dimensions (a convolution's weight) counts as [first, all the others].
     scale: 'shape' s = sqrt(max(1, rows / cols)), 'rms' s = 0.2 sqrt(max(rows, cols)) (the size of an Adam step), None s = 1.
-    Up to 32 matrices share each launch of the tiled products; those that fit one workgroup's LDS take one launch of
-    their own, or join the others where that is less work.  steps, coefficients, eps, arithmetic: as for `orthogonalize`."""
+    Up to 32 matrices share each launch of the tiled products; small ones, a workgroup each, take one launch of their
+    own, or join the others where that is less work.  steps, coefficients, eps, arithmetic: as for `orthogonalize`."""
     params, grads, momenta = list(params), list(grads), list(momenta)
     if not len(params) == len(grads) == len(momenta):
         raise RuntimeError(f"muon_step: {len(params)} parameters, {len(grads)} gradients, {len(momenta)} momenta")

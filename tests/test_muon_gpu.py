@@ -69,6 +69,20 @@ def test_large_matrices(shape, dtype):
     assert float((y.double() - want).norm() / want.norm()) <= TOL[dtype]
 
 
+# matrices of two and three blocks per wave go to one workgroup each from 256 of them on; the same ones alone do not
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(256, 60, 500), (259, 30, 1180), (256, 1180, 30)], ids=str)
+def test_large_batches_of_middling_matrices(shape, dtype):
+    x = gaussian(*shape, seed=3, dtype=dtype)
+    y = ops.orthogonalize(x.to(DEV))
+    some = [0, 17, shape[0] - 1]
+    want = exact(x[some])
+    for i, k in enumerate(some):
+        assert off(y[k], want[i]) <= TOL[dtype]
+        assert off(ops.orthogonalize(x[k].to(DEV)), want[i]) <= TOL[dtype]
+    assert bool(torch.isfinite(y).all())
+
+
 @pytest.mark.parametrize("steps", [1, 2, 3, 9, 16])
 @pytest.mark.parametrize("shape", [(40, 70), (150, 260)], ids=str)
 def test_number_of_steps(shape, steps):
