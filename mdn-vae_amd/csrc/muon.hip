@@ -1119,11 +1119,11 @@ struct MuPlan {
 // CU is bound by its own chain of loads, reads and products; where more share a CU their products add up, and the fullest CU
 // decides.  A 128 x 128 tile is four times the work of 64 x 64 for two to three times the time of a step, but starts and ends
 // more slowly and leaves CUs idle sooner.  The numbers are a fit to products of 160 x 1000 to 4 x 1024 x 2048, each tile and 1 to
-// 12 splits measured.  With 64 and with 128 (five iterations, fp32): 160 x 1000 126 and 140 us, 1000 x 1000 214 and 225,
-// 1024 x 2048 276 and 275, 2000 x 2000 737 and 662.
+// 12 splits measured.  With 64 and with 128 (five iterations, fp32): 160 x 1000 112 and 127 us, 1000 x 1000 200 and 209, 1024 x 4624
+// 440 and 435, 4 x 1024 x 2048 681 and 628, 2000 x 2000 759 and 687.
 static double mu_cost(double wgs, double ks, int tile, int terms) {
     const double n = wgs / MU_CUS, whole = n > 4 ? n + 0.5 : std::ceil(n);       // from the fifth on they even out
-    if (tile == 64) return terms == 3 ? ks * std::max(0.13, 0.115 * whole) : ks * std::max(0.11, 0.07 * whole);
+    if (tile == 64) return terms == 3 ? ks * std::max(0.13, 0.125 * whole) : ks * std::max(0.11, 0.07 * whole);
     const double full = std::ceil(n);
     if (terms == 3) return 3.0 + ks * (n <= 1 ? 0.22 + 0.12 * n : 0.30 * full);
     return 2.4 + ks * (n <= 1 ? 0.13 + 0.07 * n : 0.137 * full);
