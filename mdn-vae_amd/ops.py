@@ -2123,6 +2123,17 @@ def _gate_call(logits, top_k, valid, want_grad):
     return loss, counts, mean_probs, n_valid, grad
 
 
+class _FirstGradient(torch.autograd.Function):
+    """A gradient under create_graph=True: refuses to be differentiated, where a plain tensor would count as a constant."""
+    @staticmethod
+    def forward(ctx, grad, x):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("gate balance loss: second derivatives are not implemented")
+
+
 class _GateBalance(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, top_k, valid):
@@ -2147,6 +2158,8 @@ class _GateBalance(torch.autograd.Function):
             call("mdnvae_gate_balance_bwd", logits.data_ptr(), ptr(valid, "valid", torch.bool), T, E, ctx.top_k, ELEMENT_TYPES[logits.dtype],
                  counts.data_ptr(), mean_probs.data_ptr(), n_valid.data_ptr(), ptr(g_loss, "g_loss"), ptr(g_mean, "g_mean"),
                  grad.data_ptr(), stream())
+        if torch.is_grad_enabled() and logits.requires_grad:
+            grad = _FirstGradient.apply(grad, logits)
         return grad, None, None
 
 
@@ -2159,7 +2172,7 @@ def gate_balance_loss(logits, top_k=1, valid=None):
     which is 1 where the rows spread evenly and grows as they agree.  loss and mean_probs are differentiable with respect to
     logits, counts are not.  A logit of -inf masks that expert out of its row (never counted), a row of nothing else is
     not valid; NaN counts as the largest number and shows in the loss.  What rows that are not valid hold is never
-    looked at, and their gradient is zero.  No valid row: zeros."""
+    looked at, and their gradient is zero.  No valid row: zeros.  Second derivatives are refused."""
     return _GateBalance.apply(logits, top_k, valid)
 
 

@@ -297,3 +297,12 @@ def test_refusals():
         for f in (ops.gate_balance_loss, ops.gate_balance_loss_and_grads):
             with pytest.raises(RuntimeError, match=match):
                 f(*bad)
+
+
+def test_second_derivatives_are_refused():
+    x = torch.randn(40, 6, device=DEV, requires_grad=True)
+    loss, _, _ = ops.gate_balance_loss(x, 2)
+    (g,) = torch.autograd.grad(loss, x, create_graph=True)
+    assert torch.equal(g.detach(), ops.gate_balance_loss_and_grads(x, 2)[3])
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        torch.autograd.grad(g.square().sum(), x)
