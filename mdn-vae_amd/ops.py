@@ -2096,6 +2096,7 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
         call("mdnvae_muon_step", pp, gp, mp, rows, cols, n, etype, float(lr), float(momentum), int(bool(nesterov)), float(weight_decay),
              UPDATE_SCALES[scale], int(steps), a, b, c, float(eps), _update_terms(arithmetic, dt),
              None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), stream())
+    torch.autograd.graph.increment_version(params + momenta)     # a backward pass that still needs the old values says so
 
 
 # ---------------------------------------------------------------------------------------

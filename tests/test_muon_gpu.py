@@ -397,3 +397,11 @@ def test_out_that_overlaps_x_is_refused():
         ops.orthogonalize(buf[:2], out=buf[1:])
     want = ops.orthogonalize(buf[:1])
     assert torch.equal(ops.orthogonalize(buf[:1], out=buf[1:2]), want)
+
+
+def test_step_between_forward_and_backward_is_noticed():
+    p, m = gaussian(40, 30).to(DEV).requires_grad_(True), torch.zeros(40, 30, device=DEV)
+    loss = (p * p).sum()
+    ops.muon_step([p], [torch.ones_like(p)], [m], lr=0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
