@@ -2043,6 +2043,7 @@ def orthogonalize(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, arithmetic
         ws = _workspace(lib.mdnvae_orthogonalize_workspace_bytes(batch, rows, cols), x.device)
         call("mdnvae_orthogonalize", xp, op, batch, rows, cols, dtype, int(steps), a, b, c, float(eps),
              _update_terms(arithmetic, x.dtype), None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), stream())
+    torch.autograd.graph.increment_version(out)          # an in-place change where it was given
     return out
 
 

@@ -405,3 +405,12 @@ def test_step_between_forward_and_backward_is_noticed():
     ops.muon_step([p], [torch.ones_like(p)], [m], lr=0.1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+def test_result_over_a_saved_tensor_is_noticed():
+    x = gaussian(40, 30).to(DEV).requires_grad_(True)
+    y = x * 2.0
+    loss = (y * y).sum()
+    ops.orthogonalize(y, out=y)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
