@@ -1093,6 +1093,10 @@ struct MuJob {                                   // one shape: `count` matrices 
 
 static long mu_up(long v, long t) { return (v + t - 1) / t * t; }
 constexpr int MU_CUS = 256;
+// A launch's extent in work-items has 32 bits, and one that passes them is not refused but runs short: what is left out stays
+// unwritten (2^24 + 3 matrices of 1 x 1, 256 threads each).
+constexpr long MU_GRID = (1L << 24) - 8;         // workgroups of 256 threads, rounded up to eight
+constexpr long MU_GRID_SMALL = (1L << 22) - 1;   // of up to 1024
 
 // Whether each matrix goes to one workgroup: X and A have to fit, and X is a block per wave, or there are matrices for all CUs.  With
 // more blocks one workgroup takes longer over them than the tiled launches do (64 x 544 87 and 78 us, an optimizer step over
@@ -1232,7 +1236,7 @@ static int mu_starts(const MuPlan& pl, int (&start)[N], F per_matrix) {
     for (int i = 0; i < N; ++i) {
         start[i] = i < pl.n ? (int)at : INT_MAX;
         if (i < pl.n) at += pl.geo[i].count * per_matrix(pl.geo[i]);
-        if (at > (1L << 30)) return 0;
+        if (at > MU_GRID) return 0;
     }
     return (int)at;
 }
@@ -1259,7 +1263,7 @@ static int mu_run_small(const MuJob* jobs, int n, const MuRun& r) {
         at += jobs[i].count;
         most = std::max(most, (mu_small_apart(g.mp, g.np) ? 8L : 4L) * g.mp * (g.np + g.mp));
         blocks = std::max(blocks, (long)(g.mp / 32) * (g.np / 32));
-        MV_REQUIRE(at <= (1L << 30), E_SHAPE, "mdnvae_orthogonalize: too many matrices for one launch");
+        MV_REQUIRE(at <= MU_GRID_SMALL, E_SHAPE, "mdnvae_orthogonalize: too many matrices for one launch");
     }
     // up to twelve blocks of X (96 x 128) leave a wave half as many registers again (68 x 68: 28 us; 32 with the 128 registers
     // that sixteen waves have)
@@ -1374,7 +1378,8 @@ static int mu_dispatch(const MuJob* jobs, int n, bool small, int dtype, int term
 // matrices of a batch that go through one pass
 static long mu_batch_per_pass(long batch, long rows, long cols, int terms) {
     MuJob j = {rows, cols, batch, nullptr, nullptr, nullptr, 0.0f};
-    if (batch == 1 || mu_small(j)) return batch;
+    if (mu_small(j)) return std::min(batch, MU_GRID_SMALL);
+    if (batch == 1) return batch;
     j.count = 1;
     MuPlan pl;
     mu_plan(&j, 1, terms, pl);                    // what one matrix takes alone: more splits than in company, if anything
@@ -1435,10 +1440,11 @@ extern "C" int mdnvae_orthogonalize(const void* x, void* out, long batch, long r
     r.decay = 0.0f;
     r.is_step = 0;
     const long per = mu_batch_per_pass(batch, rows, cols, terms), size = dtype == MDNVAE_F32 ? 4 : 2;
+    const bool small = mu_small(MuJob{rows, cols, batch, nullptr, nullptr, nullptr, 0.0f});     // of all passes, as the workspace is
     for (long at = 0; at < batch; at += per) {
         MuJob j = {rows, cols, std::min(per, batch - at), static_cast<char*>(out) + at * rows * cols * size,
                    static_cast<const char*>(x) + at * rows * cols * size, nullptr, 0.0f};
-        const int rc = mu_dispatch(&j, 1, mu_small(j), dtype, terms, r, static_cast<char*>(workspace));
+        const int rc = mu_dispatch(&j, 1, small, dtype, terms, r, static_cast<char*>(workspace));
         if (rc) return rc;
     }
     return 0;
