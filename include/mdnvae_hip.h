@@ -708,8 +708,8 @@ int mdnvae_graph_features(const float* mats, long count, int n, int weighted_pat
  *     X = G / max(|G|_F, eps) (transposed if rows > cols);  `steps` times: A = X X^T, X <- a X + (b A + c A^2) X
  * out = X in G's shape and type.  x, out: [batch][rows][cols], fp32 or bf16 (`dtype`); out may be x but not overlap it
  * otherwise.  A matrix that holds a NaN or an infinity gives NaN throughout; a zero matrix gives zeros.  terms = 3:
- * fp32-level products (two fp16 parts per operand), 1: one product of the high parts (about 1e-3 of the result's norm:
- * for 16-bit results); matrices that one workgroup takes (small ones) always have the former.  Coefficients that could take a singular
+ * fp32-level products (two fp16 parts per operand), 1: one product of the high parts, 1e-3 to 2e-3 of the result's norm
+ * for a third of the work; matrices that one workgroup takes (small ones) always have the former.  Coefficients that could take a singular
  * value in [0, 1] past 256 are refused.  Workspace: 256-byte aligned, sized by the query (0 where each matrix takes one
  * workgroup). */
 enum { MDNVAE_F32 = 0, MDNVAE_BF16 = 1 };

@@ -1989,12 +1989,10 @@ def _element_type(t, name):
     return ELEMENT_TYPES[t.dtype]
 
 
-def _update_terms(arithmetic, dtype):
-    if arithmetic is None:
-        return 3 if dtype == torch.float32 else 1
-    if arithmetic not in ("f16x2", "f16"):
+def _update_terms(arithmetic):
+    if arithmetic not in (None, "f16x2", "f16"):
         raise ValueError(f"arithmetic {arithmetic!r}: 'f16x2' (two fp16 parts per operand) or 'f16' (the high part)")
-    return 3 if arithmetic == "f16x2" else 1
+    return 1 if arithmetic == "f16" else 3
 
 
 def _workspace(nbytes, device):
@@ -2015,8 +2013,9 @@ def orthogonalize(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, arithmetic
     transposed matrix if m > n).  Same shape and type as x; `out` may be given and may be x, but not overlap it otherwise.
     Not differentiable.
 
-    arithmetic: 'f16x2' (default for fp32) products from two fp16 parts per operand, fp32-level; 'f16' (default for
-    bf16) one product of the high parts, about 1e-3 of the result's norm, a third of the work.  Small matrices (up to
+    arithmetic: 'f16x2' (default) products from two fp16 parts per operand, fp32-level for both types: a bf16 result is the
+    fp32 one rounded once.  'f16': one product of the high parts, 1e-3 to 2e-3 of the result's norm (as much again as the
+    rounding of a bf16 result), a third of the work.  Small matrices (up to
     128 x 128, or 16384 entries padded to 32; somewhat larger ones in batches of hundreds) take one workgroup each, are bound by
     latency and always have 'f16x2'.
     A matrix that holds a NaN or an infinity becomes NaN throughout (the others of the batch do not), a zero matrix
@@ -2042,7 +2041,7 @@ def orthogonalize(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, arithmetic
     with _on(x.device):
         ws = _workspace(lib.mdnvae_orthogonalize_workspace_bytes(batch, rows, cols), x.device)
         call("mdnvae_orthogonalize", xp, op, batch, rows, cols, dtype, int(steps), a, b, c, float(eps),
-             _update_terms(arithmetic, x.dtype), None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), stream())
+             _update_terms(arithmetic), None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), stream())
     torch.autograd.graph.increment_version(out)          # an in-place change where it was given
     return out
 
@@ -2095,7 +2094,7 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
     with _on(dev):
         ws = _workspace(lib.mdnvae_muon_workspace_bytes(rows, cols, n), dev)
         call("mdnvae_muon_step", pp, gp, mp, rows, cols, n, etype, float(lr), float(momentum), int(bool(nesterov)), float(weight_decay),
-             UPDATE_SCALES[scale], int(steps), a, b, c, float(eps), _update_terms(arithmetic, dt),
+             UPDATE_SCALES[scale], int(steps), a, b, c, float(eps), _update_terms(arithmetic),
              None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), stream())
     torch.autograd.graph.increment_version(params + momenta)     # a backward pass that still needs the old values says so
 

@@ -1,4 +1,5 @@
-"""Orthogonalised updates: calls that once went wrong (batches of more matrices than one launch's extent holds)."""
+"""Orthogonalised updates: calls that once went wrong (batches of more matrices than one launch's extent holds,
+bf16 results with products of fewer bits than asked for)."""
 import pytest
 import torch
 
@@ -39,3 +40,26 @@ def test_more_small_matrices_than_a_launch_holds(count, rows, cols, dtype):
         e = exact(one[k])
         assert float((want[k].double().cpu() - e).norm()) <= (half + TOL32) * float(e.norm())
         assert bool((y[k::8] == want[k]).all()), k
+
+
+# both tiles, shares of X X^T, one workgroup, a batch
+@pytest.mark.parametrize("shape", [(68, 68), (64, 512), (129, 129), (192, 1728), (1024, 640), (640, 1024), (1000, 4624), (16, 160, 161)], ids=str)
+def test_bf16_result_is_the_fp32_one_rounded_once(shape):
+    x = gaussian(*shape, seed=1, dtype=torch.bfloat16).to(DEV)
+    wide = ops.orthogonalize(x.float())
+    assert torch.equal(ops.orthogonalize(x), wide.bfloat16())
+    # and so is as near to the definition as its rounding lets it be: |got - e| <= |rounded(e) - e| + 2 |fp32 result - e|
+    e = exact(x)
+    own = float((e.bfloat16().double() - e).norm())
+    assert float((ops.orthogonalize(x).double().cpu() - e).norm()) <= own + 2 * TOL32 * float(e.norm())
+
+
+def test_bf16_step_is_the_fp32_one_rounded_once():
+    shapes = [(48, 1, 7, 7), (96, 48, 3, 3), (192, 96, 3, 3), (192, 192, 3, 3), (68, 768), (5, 4)]
+    p, g = ([gaussian(*s, seed=k + i, dtype=torch.bfloat16).to(DEV) for i, s in enumerate(shapes)] for k in (0, 50))
+    m = [gaussian(*s, seed=90 + i).to(DEV) for i, s in enumerate(shapes)]
+    wide = [[t.float() for t in ts] for ts in (p, g)] + [[t.clone() for t in m]]
+    ops.muon_step(p, g, m, lr=0.5, weight_decay=0.1)
+    ops.muon_step(*wide, lr=0.5, weight_decay=0.1)
+    assert all(torch.equal(a, b.bfloat16()) for a, b in zip(p, wide[0]))
+    assert all(torch.equal(a, b) for a, b in zip(m, wide[2]))
