@@ -1455,7 +1455,8 @@ extern "C" int mdnvae_orthogonalize(const void* x, void* out, long batch, long r
 // the first result that is not 0.  Matrices that fit one workgroup are a group of their own, unless there are others, one group
 // holds all and the plan for it takes 64 x 64 tiles: then their tiles cost the launches of the others less than a launch of
 // their own (a convolutional encoder's list of 192 x 1728 and smaller ones in bf16 200 -> 177 us).  A 128 x 128 tile is too much
-// for them (the gated mixture's 1077 -> 1095 us).
+// for them (the gated mixture's 1077 -> 1095 us).  With one term per product they stay apart: a workgroup of their own keeps both
+// parts, and what else is in the list must not take them away.
 template <typename F>
 static int mu_groups(const long* rows, const long* cols, int count, int terms, F f) {
     MuJob every[MU_MAX];
@@ -1468,7 +1469,7 @@ static int mu_groups(const long* rows, const long* cols, int count, int terms, F
         ++all;
     }
     bool together = false;
-    if (tiled > 0 && tiled < all && all <= MU_MAX) {
+    if (terms == 3 && tiled > 0 && tiled < all && all <= MU_MAX) {
         MuPlan pl;
         mu_plan(every, all, terms, pl);
         together = pl.tile == 64;

@@ -2066,7 +2066,8 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
     one device.  A tensor of more than two dimensions (a convolution's weight) counts as [first, all the others].
     scale: 'shape' s = sqrt(max(1, rows / cols)), 'rms' s = 0.2 sqrt(max(rows, cols)) (the size of an Adam step), None s = 1.
     Up to 32 matrices share each launch of the tiled products; small ones, a workgroup each, take one launch of their
-    own, or join the others where that is less work.  steps, coefficients, eps, arithmetic: as for `orthogonalize`."""
+    own, or join the others where that is less work and the arithmetic 'f16x2' (fp32-level either way; the last bits may differ).
+    steps, coefficients, eps, arithmetic: as for `orthogonalize`, small matrices always 'f16x2'."""
     params, grads, momenta = list(params), list(grads), list(momenta)
     if not len(params) == len(grads) == len(momenta):
         raise RuntimeError(f"muon_step: {len(params)} parameters, {len(grads)} gradients, {len(momenta)} momenta")

@@ -1,5 +1,5 @@
 """Orthogonalised updates: calls that once went wrong (batches of more matrices than one launch's extent holds,
-bf16 results with products of fewer bits than asked for)."""
+bf16 results with products of fewer bits than asked for, small matrices whose arithmetic their neighbours decided)."""
 import pytest
 import torch
 
@@ -63,3 +63,22 @@ def test_bf16_step_is_the_fp32_one_rounded_once():
     ops.muon_step(*wide, lr=0.5, weight_decay=0.1)
     assert all(torch.equal(a, b.bfloat16()) for a, b in zip(p, wide[0]))
     assert all(torch.equal(a, b) for a, b in zip(m, wide[2]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("arithmetic", ["f16", "f16x2"])
+def test_a_small_matrix_keeps_its_arithmetic_in_any_company(arithmetic, dtype):
+    """The large ones take 64 x 64 tiles: the list that the small ones would join."""
+    shapes = [(68, 68), (48, 49), (128, 128), (1, 9), (192, 1728), (192, 1728), (192, 900)]
+    make = lambda k, n: [gaussian(*s, seed=k + i, dtype=dtype).to(DEV) for i, s in enumerate(shapes[:n])]  # noqa: E731
+    zeros = lambda n: [torch.zeros(s, device=DEV) for s in shapes[:n]]  # noqa: E731
+    p = [torch.zeros_like(t) for t in make(0, 7)]
+    alone = [t.clone() for t in p[:4]]
+    ops.muon_step(p, make(50, 7), zeros(7), lr=1.0, scale=None, arithmetic=arithmetic)
+    ops.muon_step(alone, make(50, 4), zeros(4), lr=1.0, scale=None, arithmetic=arithmetic)
+    half = 0.0 if dtype == torch.float32 else 2.0 ** -8
+    for a, b, g in zip(p, alone, make(50, 4)):
+        e = exact(g)                                                     # u = g + 0.95 g: a multiple
+        assert float((a.double().cpu() + e).norm()) <= (half + TOL32) * float(e.norm())
+        if arithmetic == "f16":
+            assert torch.equal(a, b)
