@@ -151,7 +151,8 @@ class Trainer:
 
     `gate_balance` (loss_mode "mdn"): adds gate_balance * batch * ops.gate_balance_loss(gate logits, gate_top_k)[0] to the
     (sum-reduced) loss, which keeps the mixture's gate from handing all subjects to one component; the counts of the last
-    step are in `gate_counts` (on the device).  With data-parallel ranks each rank balances its own shard."""
+    step, eager or replayed, are in `gate_counts` (on the device; a replay's last until the next one).  With data-parallel
+    ranks each rank balances its own shard."""
 
     def __init__(self, model, loss_mode, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, group=None, fused_loss=True,
                  overlap_floats=1 << 20, direct_grads=True, folded_adam=True, fast_wgrad=False, optimizer="adam", muon_lr=0.02,
@@ -418,6 +419,7 @@ class Trainer:
         state = [self.buf.flat_p, self.exp_avg, self.exp_avg_sq, self.muon_buf] + list(self._fold_m.values()) + \
             list(self._fold_v.values())
         keep = [t.clone() for t in state]
+        counts = self.gate_counts
 
         def backward_part():
             return self.forward_backward(self._g_inputs, self._g_target, self._g_eps, _defer_fold=True)
@@ -449,6 +451,8 @@ class Trainer:
                     adam_part()
         finally:
             self._split_graph = False
+            # the graph's own counts hold nothing until a replay has written them
+            self._g_gate_counts, self.gate_counts = self.gate_counts, counts
         for dst, src in zip(state, keep):
             dst.copy_(src)
         self._g_step.fill_(self.steps)
@@ -474,6 +478,8 @@ class Trainer:
             self._graph_adam.replay()
         self.steps += 1
         self._g_step_holds = self.steps
+        if self.gate_balance:
+            self.gate_counts = self._g_gate_counts
         return self._g_loss
 
     def hinge_step(self, fc, sc, eps_with=None, eps_without=None, generator=None, margin=0.01):
