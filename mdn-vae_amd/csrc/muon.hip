@@ -1046,7 +1046,9 @@ static bool mu_scales(const MuCoef& co, MuSteps& st, float& x0_scale) {
     const double a = co.a, b = co.b, c = co.c;
     double s = 1.0;
     st.steps = co.steps;
-    auto scale = [](double bound) { return std::exp2(std::floor(std::log2(32768.0 / std::max(bound, 1e-3)))); };
+    // the least bound is far below what coefficients that shrink X come to (0.1, 0, 0 in sixteen steps: 1e-16), so that X stays in
+    // the middle of fp16's range with them too; the factors below stay inside fp32
+    auto scale = [](double bound) { return std::exp2(std::floor(std::log2(32768.0 / std::max(bound, 1e-36)))); };
     double sx = scale(s);
     x0_scale = (float)sx;
     for (int k = 0; k < co.steps; ++k) {

@@ -1,5 +1,6 @@
 """Orthogonalised updates: calls that once went wrong (batches of more matrices than one launch's extent holds,
-bf16 results with products of fewer bits than asked for, small matrices whose arithmetic their neighbours decided)."""
+bf16 results with products of fewer bits than asked for, small matrices whose arithmetic their neighbours decided,
+coefficients that shrink the iterates below what fp16 parts held)."""
 import pytest
 import torch
 
@@ -82,3 +83,15 @@ def test_a_small_matrix_keeps_its_arithmetic_in_any_company(arithmetic, dtype):
         assert float((a.double().cpu() + e).norm()) <= (half + TOL32) * float(e.norm())
         if arithmetic == "f16":
             assert torch.equal(a, b)
+
+
+# one block of X per wave (kept in fp32 registers), two and three blocks, tiled
+@pytest.mark.parametrize("shape", [(40, 70), (256, 60, 500), (256, 30, 1180), (150, 260), (1000, 1000)], ids=str)
+@pytest.mark.parametrize("coefficients,steps", [((0.1, 0.0, 0.0), 16), ((0.2, 0.1, 0.0), 16), ((0.05, 0.3, -0.2), 12), ((0.01, 0.0, 0.0), 16),
+                                                ((0.5, 0.0, 0.0), 3), ((0.0, 0.0, 0.0), 2)], ids=str)
+def test_coefficients_that_shrink_the_iterates(shape, coefficients, steps):
+    x = gaussian(*shape, seed=4).to(DEV)
+    got, want = ops.orthogonalize(x, steps=steps, coefficients=coefficients), exact(x[:2] if len(shape) == 3 else x, steps, coefficients)
+    got = (got[:2] if len(shape) == 3 else got).double().cpu()
+    # three roundings a step, as everywhere: nothing here is amplified
+    assert float((got - want).norm()) <= 12 * steps * 2.0 ** -22 * float(want.norm())
