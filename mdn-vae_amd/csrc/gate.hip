@@ -11,7 +11,8 @@
 //
 // Two sweeps over the logits, since every gradient depends on the counts of all rows: statistics, then gradient.  A row
 // belongs to a group of L lanes, eight (sixteen above 128 experts) values each; experts stay with their lane, so sums of
-// p and counts are kept in registers over all rows of a wave and leave once per workgroup.  Selection: every lane sorts its
+// p and counts are kept in registers over the rows of a wave.  Sums of p are fp32 over at most 32 rows of a lane and the groups
+// of its wave; from there on float64, for equal rows round alike and their errors add up (512 rows of a lane: 6e-6).  Selection: every lane sorts its
 // keys once (a network of 19 or 63 exchanges), then k rounds of "largest head of the group, its lane moves on" find the
 // k-th largest key; whoever is above it is taken, and of those equal to it as many of the lowest index as are
 // missing (ballots; only where the group saw a tie).  Sixteen lanes of sixteen values rather than thirty-two of eight for 256
@@ -234,9 +235,12 @@ struct GateArgs {
 };
 
 // rows [first, T) in steps of `stride` of this group: its lanes' sums of p, counts, and the number of valid rows.  The trip
-// count is that of the whole wave (ballots), rows past the end count as padding.
-template <typename T, int L, int NV, int VEC>
-__device__ __forceinline__ void gt_stats(const GateArgs& a, long wave_first, long stride, float (&ps)[NV], int (&cn)[NV], int& rows) {
+// count is that of the whole wave (ballots), rows past the end count as padding.  flush(): takes the sums of p and sets them to
+// zero, after every GT_FLUSH rows of a lane.
+constexpr int GT_FLUSH = 32;
+template <typename T, int L, int NV, int VEC, typename FLUSH>
+__device__ __forceinline__ void gt_stats(const GateArgs& a, long wave_first, long stride, float (&ps)[NV], int (&cn)[NV], int& rows,
+                                         FLUSH flush) {
     const int lane = threadIdx.x & 63, l = lane & (L - 1), gr = lane / L;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -252,6 +256,7 @@ __device__ __forceinline__ void gt_stats(const GateArgs& a, long wave_first, lon
         gt_load<T, L, NV, VEC>(logits + (in ? r : 0) * a.E, a.E, l, in, d);
     };
     if (wave_first < a.T) fetch(wave_first, z);
+    int held = 0;
     for (long r0 = wave_first; r0 < a.T; r0 += stride) {
         if (r0 + stride < a.T) fetch(r0 + stride, next);           // under this row's arithmetic
         unsigned key[NV];
@@ -264,21 +269,26 @@ __device__ __forceinline__ void gt_stats(const GateArgs& a, long wave_first, lon
             cn[v] += key[v] >= floor_key ? 1 : 0;
             z[v] = next[v];
         }
+        if (++held == GT_FLUSH) {
+            flush();
+            held = 0;
+        }
     }
 }
 
 // sums over the groups of a wave
-template <int L, int NV>
-__device__ __forceinline__ void gt_wave_total(float (&ps)[NV], int (&cn)[NV], int& rows) {
+template <int L, int NV, typename N>
+__device__ __forceinline__ void gt_wave_total(N (&s)[NV]) {
 #pragma unroll
-    for (int o = L; o < 64; o <<= 1) {
+    for (int o = L; o < 64; o <<= 1)
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            ps[v] += __shfl_xor(ps[v], o, 64);
-            cn[v] += __shfl_xor(cn[v], o, 64);
-        }
-        rows += __shfl_xor(rows, o, 64);
-    }
+        for (int v = 0; v < NV; ++v) s[v] += __shfl_xor(s[v], o, 64);
+}
+template <int L>
+__device__ __forceinline__ int gt_wave_total(int rows) {
+#pragma unroll
+    for (int o = L; o < 64; o <<= 1) rows += __shfl_xor(rows, o, 64);
+    return rows;
 }
 
 // gradient of the same rows; w: the lane's weights
@@ -327,34 +337,52 @@ __device__ __forceinline__ float gt_weight(int count, double count_mean, int n, 
 
 constexpr int GT_NT = 256;
 
-// sweep 1: one partial row of sums and counts per workgroup
+// sweep 1: one partial row of sums and counts per workgroup.  Four waves per SIMD, one for each workgroup that a CU gets; with
+// thirty-two lanes per row that would take spills of 12 to 120 registers, and three it is.
 template <typename T, int L, int NV, int VEC>
-__global__ __launch_bounds__(GT_NT) void gate_stats_kernel(GateArgs a, float* __restrict__ part_p, int* __restrict__ part_c,
+__global__ __launch_bounds__(GT_NT, L == 32 ? 3 : 4) void gate_stats_kernel(GateArgs a, float* __restrict__ part_p, int* __restrict__ part_c,
                                                            int* __restrict__ part_n) {
-    __shared__ float sp[GT_NT / 64][L * NV];
-    __shared__ int sc[GT_NT / 64][L * NV];
+    __shared__ union {                                     // one after the other
+        double sums[GT_NT / 64][L * NV];
+        int counts[GT_NT / 64][L * NV];
+    } table;
+    auto& sp = table.sums;
+    auto& sc = table.counts;
     __shared__ int sn[GT_NT / 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     constexpr int G = 64 / L;
     float ps[NV];
     int cn[NV], rows;
     const long stride = (long)gridDim.x * (GT_NT / 64) * G;
-    gt_stats<T, L, NV, VEC>(a, ((long)blockIdx.x * (GT_NT / 64) + wave) * G, stride, ps, cn, rows);
-    gt_wave_total<L, NV>(ps, cn, rows);
-    if (lane < L) {
+    if (lane < L) {                                        // a lane's entries are its own until the barrier
+#pragma unroll
+        for (int v = 0; v < NV; ++v) sp[wave][GateMap<L, NV, VEC>::at(lane, v)] = 0.0;
+    }
+    auto flush = [&] {
+        gt_wave_total<L, NV>(ps);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            sp[wave][GateMap<L, NV, VEC>::at(lane, v)] = ps[v];
-            sc[wave][GateMap<L, NV, VEC>::at(lane, v)] = cn[v];
+            if (lane < L) sp[wave][GateMap<L, NV, VEC>::at(lane, v)] += (double)ps[v];
+            ps[v] = 0.0f;
         }
-    }
+    };
+    gt_stats<T, L, NV, VEC>(a, ((long)blockIdx.x * (GT_NT / 64) + wave) * G, stride, ps, cn, rows, flush);
+    flush();
+    gt_wave_total<L, NV>(cn);
+    rows = gt_wave_total<L>(rows);
     if (lane == 0) sn[wave] = rows;
     __syncthreads();
-    for (int e = threadIdx.x; e < a.E; e += GT_NT) {
-        part_p[(long)blockIdx.x * a.E + e] = (sp[0][e] + sp[1][e]) + (sp[2][e] + sp[3][e]);
-        part_c[(long)blockIdx.x * a.E + e] = (sc[0][e] + sc[1][e]) + (sc[2][e] + sc[3][e]);
-    }
+    for (int e = threadIdx.x; e < a.E; e += GT_NT)
+        part_p[(long)blockIdx.x * a.E + e] = (float)((sp[0][e] + sp[1][e]) + (sp[2][e] + sp[3][e]));
     if (threadIdx.x == 0) part_n[blockIdx.x] = (sn[0] + sn[1]) + (sn[2] + sn[3]);
+    __syncthreads();
+    if (lane < L) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) sc[wave][GateMap<L, NV, VEC>::at(lane, v)] = cn[v];
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.E; e += GT_NT)
+        part_c[(long)blockIdx.x * a.E + e] = (sc[0][e] + sc[1][e]) + (sc[2][e] + sc[3][e]);
 }
 
 // the workgroups' rows summed: 16 experts per workgroup, 64 threads each, float64, fixed order
@@ -508,8 +536,10 @@ __global__ __launch_bounds__(GT_ONE_NT) void gate_one_kernel(GateArgs a, float* 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & (L - 1);
     float ps[NV];
     int cn[NV], rows;
-    gt_stats<T, L, NV, VEC>(a, (long)wave * G, (long)W * G, ps, cn, rows);
-    gt_wave_total<L, NV>(ps, cn, rows);
+    gt_stats<T, L, NV, VEC>(a, (long)wave * G, (long)W * G, ps, cn, rows, [] {});      // eight rows of a lane at most: gt_one
+    gt_wave_total<L, NV>(ps);
+    gt_wave_total<L, NV>(cn);
+    rows = gt_wave_total<L>(rows);
     if (lane < L) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {

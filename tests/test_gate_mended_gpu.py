@@ -1,4 +1,4 @@
-"""Balance loss of a gate: calls that once went wrong (a trainer's counts after replays)."""
+"""Balance loss of a gate: calls that once went wrong (a trainer's counts after replays, means over very many rows)."""
 import pytest
 import torch
 
@@ -46,3 +46,32 @@ def test_gate_counts_are_the_last_steps_eager_or_replayed(fused, optimizer):
     trainer.capture((x[b], adjacency, traits[b]), x[b], eps[b])
     assert trainer.gate_counts is held                       # capturing is no step
     run(trainer.replay, b)
+
+
+# probabilities carry about eight fp32 roundings, and their sum eight more: sixteen halves of a step, whatever the number of rows
+@pytest.mark.parametrize("T,E,dtype", [(1 << 27, 5, torch.float32), (1 << 26, 5, torch.float32), (1 << 25, 60, torch.bfloat16),
+                                       (1 << 23, 160, torch.bfloat16), (1 << 21, 1000, torch.bfloat16), (1 << 21, 500, torch.float32)])
+def test_means_over_many_equal_rows(T, E, dtype):
+    """Every row rounds the same way: 128 to 512 rows of a lane in one fp32 sum were off by up to 6e-6."""
+    loss, counts, mean = M.gate_balance_loss(torch.zeros(T, E, dtype=dtype, device=DEV), 1)
+    assert int(counts[0]) == T and int(counts.sum()) == T
+    assert float((mean.double() * E - 1.0).abs().max()) <= 16 * 2.0 ** -24
+    assert abs(float(loss) - 1.0) <= 2 * 16 * 2.0 ** -24
+
+
+def test_rows_of_a_lane_on_both_sides_of_a_flush():
+    """1024 workgroups of 4 waves: one row per lane and 4096, 8192, ... rows more; padding in between."""
+    E = 513                                                   # a row per wave
+    for rows in (31, 32, 33, 64, 70):
+        T = 4096 * (rows - 1) + 5
+        z = torch.randn(T, E, generator=torch.Generator(device=DEV).manual_seed(rows), device=DEV)
+        valid = torch.rand(T, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV) < 0.9
+        loss, counts, mean = M.gate_balance_loss(z, 1, valid)
+        n = int(valid.sum())
+        want = torch.zeros(E, dtype=torch.float64, device=DEV)
+        for lo in range(0, T, 1 << 16):
+            want += (torch.softmax(z[lo:lo + (1 << 16)].double(), dim=1) * valid[lo:lo + (1 << 16), None]).sum(dim=0)
+        assert torch.equal(counts.long(), torch.bincount(z[valid].argmax(dim=1), minlength=E))
+        assert float((mean.double() * n / want - 1.0).abs().max()) <= 16 * 2.0 ** -24, rows
+        want_loss = float(E / n * (counts.double() * want / n).sum())
+        assert abs(float(loss) - want_loss) <= 2 * 16 * 2.0 ** -24 * want_loss
