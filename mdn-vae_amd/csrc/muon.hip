@@ -364,7 +364,8 @@ constexpr int MU_RING = 5;
 // early(): EXTRA loads into registers that the epilogue wants, issued eight steps before the end and not behind it (B X at
 // 4624 x 4624 590 -> 576 us).
 // The counted waits rely on exactly EXTRA loads: mu_load_block's are eight bytes each, no two of a lane
-// adjacent (half tiles lie 16 bytes apart in an order that depends on the row, parts 1 KiB), so none can be joined.
+// adjacent (half tiles lie 16 bytes apart in an order that depends on the row, parts 1 KiB), so none can be joined.  A CPU test
+// counts them in the built library.
 template <int TILE, int TERMS, bool TR, int EXTRA, typename EARLY>
 __device__ __forceinline__ void mu_mainloop(const char* rsrc, const char* csrc, int nsteps, int KS, int k0, int k1, char* smem,
                                             mu_acc (&acc)[TILE / 64][TILE / 64], EARLY early) {
