@@ -147,7 +147,7 @@ class Trainer:
     `optimizer`: "adam" (the reference's) or "muon": weights of two and more dimensions (a convolution's as [out, rest])
     take orthogonalised momentum updates (ops.muon_step with `muon_lr`, `muon_momentum`, `muon_nesterov`,
     `muon_weight_decay`), all other parameters Adam with `lr`.  `muon_params(name, parameter) -> bool` chooses otherwise.
-    Gradients of symmetric-input first layers are unfolded for it (`folded_adam` is an Adam layout).
+    Gradients of symmetric-input first layers are unfolded for it (`folded_adam` is an Adam layout).  Masked weights stay zero.
 
     `gate_balance` (loss_mode "mdn"): adds gate_balance * batch * ops.gate_balance_loss(gate logits, gate_top_k)[0] to the
     (sum-reduced) loss, which keeps the mixture's gate from handing all subjects to one component; the counts of the last
@@ -208,6 +208,8 @@ class Trainer:
         views = [(o, p) for o, p in zip(self.buf.offsets, self.buf.params[:len(muon)])]
         self._muon_views = [[flat[o:o + p.numel()].view(p.shape) for o, p in views]
                             for flat in (self.buf.flat_p, self.buf.flat_g, self.muon_buf)]
+        # an orthogonalised update is not zero where its gradient is: masked weights are put back to zero after it
+        self._muon_masked = [m for m in model.modules() if hasattr(m, "mask_flag") and id(getattr(m, "weight", None)) in muon]
         self._defer_fold = False    # inside step(): folded gradients are not unfolded into .grad
         self.steps = 0
         self.fused_loss = fused_loss
@@ -378,6 +380,9 @@ class Trainer:
         lo = max(self._fold_end, self._muon_end)
         if self._muon_end:
             ops.muon_step(*self._muon_views, **self.muon)
+            for m in self._muon_masked:
+                if m.mask_flag:
+                    m.weight.data.mul_(m.mask)
         args = (float(self.lr), float(self.betas[0]), float(self.betas[1]), float(self.eps), 1.0, stream())
         rest = (ptr(self.buf.flat_p[lo:]), ptr(self.buf.flat_g[lo:]), ptr(self.exp_avg[lo:]), ptr(self.exp_avg_sq[lo:]),
                 self.buf.numel - lo)

@@ -1,9 +1,10 @@
 """Orthogonalised updates: calls that once went wrong (batches of more matrices than one launch's extent holds,
 bf16 results with products of fewer bits than asked for, small matrices whose arithmetic their neighbours decided,
-coefficients that shrink the iterates below what fp16 parts held)."""
+coefficients that shrink the iterates below what fp16 parts held, masked weights)."""
 import pytest
 import torch
 
+import mdnvae_amd as M
 from mdnvae_amd import ops
 
 pytestmark = pytest.mark.gpu
@@ -95,3 +96,28 @@ def test_coefficients_that_shrink_the_iterates(shape, coefficients, steps):
     got = (got[:2] if len(shape) == 3 else got).double().cpu()
     # three roundings a step, as everywhere: nothing here is amplified
     assert float((got - want).norm()) <= 12 * steps * 2.0 ** -22 * float(want.norm())
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_masked_weights_stay_zero(graph):
+    """A masked layer's gradient is zero where its mask is, its orthogonalised update is not."""
+    torch.manual_seed(3)
+    n, B = 68, 4
+    model = M.ConvVAE(decoder="gcn", intercept="diag", final="none", n_nodes=n, latent_dim=68).to(DEV)
+    x, eps = M.data.synthetic_sc(B, n, seed=4, device=DEV), torch.randn(B, 68, device=DEV)
+    trainer = M.Trainer(model, "poisson_log", optimizer="muon", muon_lr=0.01)
+    mask = (torch.rand(n, n) < 0.5).float().fill_diagonal_(1.0)
+    model.set_mask([mask] * 5)
+    names = [f"fc{i}.weight" for i in range(4, 9)]
+    before = {k: v.detach().clone() for k, v in model.named_parameters() if k in names}
+    if graph:
+        trainer.capture((x,), x, eps)
+    for _ in range(2):
+        (trainer.replay if graph else trainer.step)((x,), x, eps)
+    torch.cuda.synchronize()
+    got = dict(model.named_parameters())
+    assert len(before) == 5
+    for k, p0 in before.items():
+        off_mask = mask.to(DEV) == 0
+        assert bool((got[k][off_mask] == 0).all()), k
+        assert bool((got[k][~off_mask] != p0[~off_mask]).float().mean() > 0.9), k
