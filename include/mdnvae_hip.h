@@ -709,9 +709,11 @@ int mdnvae_graph_features(const float* mats, long count, int n, int weighted_pat
  * out = X in G's shape and type.  x, out: [batch][rows][cols], fp32 or bf16 (`dtype`); out may be x but not overlap it
  * otherwise.  A matrix that holds a NaN or an infinity gives NaN throughout; a zero matrix gives zeros.  terms = 3:
  * fp32-level products (two fp16 parts per operand), 1: one product of the high parts, 1e-3 to 2e-3 of the result's norm
- * for a third of the work; matrices that one workgroup takes (small ones) always have the former.  Coefficients that could take a singular
- * value in [0, 1] past 256 are refused.  Workspace: 256-byte aligned, sized by the query (0 where each matrix takes one
- * workgroup). */
+ * for a third of the work; matrices that one workgroup takes (small ones) always have the former.  Coefficients are refused
+ * that could take a singular value in [0, 1] past 16 before the last step or 256 after it, or one of b A + c A^2 past 256.
+ * Roundings are relative to the most that the coefficients let a singular value become; X_0 is exact to 2^-40, which for a
+ * matrix of a norm far below eps is a share of sqrt(rows cols) 2^-40 eps / |G|_F.  Workspace: 256-byte aligned, sized by the
+ * query (0 where each matrix takes one workgroup). */
 enum { MDNVAE_F32 = 0, MDNVAE_BF16 = 1 };
 enum { MDNVAE_MUON_MAX_STEPS = 16 };
 size_t mdnvae_orthogonalize_workspace_bytes(long batch, long rows, long cols);

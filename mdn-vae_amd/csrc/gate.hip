@@ -12,10 +12,10 @@
 // Two sweeps over the logits, since every gradient depends on the counts of all rows: statistics, then gradient.  A row
 // belongs to a group of L lanes, eight (sixteen above 128 experts) values each; experts stay with their lane, so sums of
 // p and counts are kept in registers over the rows of a wave.  Sums of p are fp32 over at most 32 rows of a lane and the groups
-// of its wave; from there on float64, for equal rows round alike and their errors add up (512 rows of a lane: 6e-6).  Selection: every lane sorts its
-// keys once (a network of 19 or 63 exchanges), then k rounds of "largest head of the group, its lane moves on" find the
-// k-th largest key; whoever is above it is taken, and of those equal to it as many of the lowest index as are
-// missing (ballots; only where the group saw a tie).  Sixteen lanes of sixteen values rather than thirty-two of eight for 256
+// of its wave; from there on float64, for equal rows round alike and their errors add up (512 rows of a lane: 6e-6).
+// Selection: every lane sorts its keys once (a network of 19 or 63 exchanges), then k rounds of "largest head of the group, its
+// lane moves on" find the k-th largest key; whoever is above it is taken, and of those equal to it as many of the lowest index
+// as are missing (ballots; only where the group saw a tie).  Sixteen lanes of sixteen values rather than thirty-two of eight for 256
 // experts: four rows per wave share each round, and all its exchanges stay within a DPP row (290 -> 95 us for 262144 rows,
 // 2.8 TB/s: bound by its instructions, about 620 per four rows).
 #include <algorithm>
@@ -71,7 +71,8 @@ __device__ __forceinline__ float gt_sum(float v) {
 }
 
 // exp(x), x <= 0 (or NaN, -inf): 2^t by the hardware with t = x log2 e rounded, and what the rounding left out as a first-order
-// factor - a couple of 2^-24 for all x, at a third of the instructions of expf
+// factor - a couple of 2^-24 for all x, at a third of the instructions of expf.  Below 2^-126 it gives zero: next to a row's largest,
+// which is 1, that is no share of its sum
 __device__ __forceinline__ float gt_exp(float x) {
     const float log2e = 1.44269504f, tail = 1.92596299e-8f, ln2 = 0.693147181f;
     const float y = fmaxf(x, -150.0f);                      // zero either way; keeps -inf out of the remainder (NaN: below)

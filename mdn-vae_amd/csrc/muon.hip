@@ -57,7 +57,7 @@ struct MuGeo {
 };
 // Kernel arguments over N entries, 1 or MU_MAX.  The arguments are in no cache yet when a kernel starts, and a round trip to
 // them is 0.6 us.  So a call over one shape has kernels of its own, without a table to look the entry up in (16 x 512 x 512 322 ->
-// 302 us, 1024 x 4624 in bf16 288 -> 267), and those over a table do so in one round trip (mu_entry).
+// 302 us, 1024 x 4624 with one term 288 -> 267), and those over a table do so in one round trip (mu_entry).
 template <int N>
 struct MuTab {
     int start[N + 1];                    // first workgroup of each entry; INT_MAX past the last
@@ -81,7 +81,7 @@ __host__ __device__ inline long mu_matrix_bytes(const MuGeo& g) {
 
 // The entry of a workgroup.  Each lane fetches one entry; which is the workgroup's is a ballot over the starts, and its values
 // come from that lane: one round trip to the arguments instead of two, starts and then the entry (a convolutional encoder's
-// list 180 -> 160 us).
+// list with one term 180 -> 160 us).
 struct MuEntry {
     MuGeo ge;
     int e, first;                        // index and first workgroup
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(256) void mu_norm_kernel(MuTab<N> tab, MuPtrs<N> pt
 }
 
 // u scale / max(|u|_F, eps) as ldexp(u, shift) * factor, since the reciprocal alone may lie outside fp32: |u|_F^2 = m 4^e with m
-// in [0.5, 2), shift = -e, factor = scale / sqrt(m).  A norm that is not finite (an infinity or a NaN in the matrix)
+// in [0.25, 1), shift = -e, factor = scale / sqrt(m).  A norm that is not finite (an infinity or a NaN in the matrix)
 // gives NaN, and with it a result that is NaN throughout.
 struct MuNorm {
     int shift;
@@ -586,7 +586,8 @@ __device__ __forceinline__ int mu_tile_index(int total) {
 }
 
 // GRAM and POLY, tiles of the upper triangle.  4624 x 4624 fp32 284 to 310 us each, 1.06 to 1.15 PFLOP/s of fp16 products (the card's
-// large library products: 1.0): the clock falls to 1.7 GHz under them, the matrix pipes are 64 % busy.  1024 x 4624 fp32 22 and 13 us.
+// large library products: 1.0): the clock falls to 1.7 GHz under them, the matrix pipes are 62 to 64 % busy.  1024 x 4624 20
+// to 22 and 13 us.
 template <int N, int TILE, int TERMS, int MODE>
 __global__ __launch_bounds__(256) void mu_sym_kernel(MuTab<N> tab, int total, char* __restrict__ ws, int ping, MuScale sc) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
@@ -686,8 +687,8 @@ __global__ __launch_bounds__(256) void mu_reduce_kernel(MuTab<N> tab, char* __re
 }
 
 // STEP: D rows = 128 (64) columns n of X, D columns = rows m, so that a lane's four consecutive rows are consecutive in X's
-// tiles.  LAST: the result leaves in the caller's layout and type.  4624 x 4624 fp32 576 to 640 us, 1.0 to 1.1 PFLOP/s; 1024 x 4624 46 us
-// (bf16 24), for 296 tiles of 128 x 128 are more than the CUs take in one round.
+// tiles.  LAST: the result leaves in the caller's layout and type.  4624 x 4624 fp32 576 to 640 us, 1.0 to 1.1 PFLOP/s; 1024 x
+// 4624 44 to 46 us on tiles of 64 x 64 (with one term 24 on 128 x 128), for 296 tiles of 128 x 128 are more than the CUs take in one round.
 template <int N, typename T, int TILE, int TERMS, bool LAST>
 __global__ __launch_bounds__(256) void mu_step_kernel(MuTab<N> tab, int total, MuPtrs<N> ptrs, char* __restrict__ ws, int ping, MuScale sc,
                                                       float decay, int is_step) {
@@ -1042,7 +1043,9 @@ struct MuCoef { int steps; float a, b, c, eps; };
 // Power-of-two scales of the iterates.  s_k bounds the singular values of X_k: s_0 = 1 and s_{k+1} is the largest
 // |s (a + b s^2 + c s^4)| on [0, s_k] (its ends and the roots of the derivative).  Entries of X are at most s_k,
 // those of A at most s_k^2, those of B at most the largest |b t + c t^2| on [0, s_k^2]; a factor of two is kept for rounding.
-// Returns false where a bound passes 256: the iteration would leave what two fp16 parts hold.
+// Returns false where one of A, B or the next X passes 256 (X itself 16, then): the iteration would leave what two fp16 parts
+// hold.  Below the bounds the parts are exact to 2^-40 of them, so a matrix whose norm is far below eps, which X_0 keeps, has that much
+// fewer bits.
 static bool mu_scales(const MuCoef& co, MuSteps& st, float& x0_scale) {
     const double a = co.a, b = co.b, c = co.c;
     double s = 1.0;
@@ -1457,7 +1460,8 @@ extern "C" int mdnvae_orthogonalize(const void* x, void* out, long batch, long r
 // The matrices of a step in order, `f(jobs, index, n, small)` for each group of up to MU_MAX that is launched together; stops at
 // the first result that is not 0.  Matrices that fit one workgroup are a group of their own, unless there are others, one group
 // holds all and the plan for it takes 64 x 64 tiles: then their tiles cost the launches of the others less than a launch of
-// their own (a convolutional encoder's list of 192 x 1728 and smaller ones in bf16 200 -> 177 us).  A 128 x 128 tile is too much
+// their own (a convolutional encoder's list of 192 x 1728 and smaller ones 191 -> 177 us in both types, of half and a quarter of
+// its widths 177 -> 134 and 140 -> 102).  A 128 x 128 tile is too much
 // for them (the gated mixture's 1077 -> 1095 us).  With one term per product they stay apart: a workgroup of their own keeps both
 // parts, and what else is in the list must not take them away.
 template <typename F>

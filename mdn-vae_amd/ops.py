@@ -2019,7 +2019,9 @@ def orthogonalize(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, arithmetic
     128 x 128, or 16384 entries padded to 32; somewhat larger ones in batches of hundreds) take one workgroup each, are bound by
     latency and always have 'f16x2'.
     A matrix that holds a NaN or an infinity becomes NaN throughout (the others of the batch do not), a zero matrix
-    stays zero.  Coefficients with which a singular value of [0, 1] could pass 256 are refused."""
+    stays zero.  Coefficients with which a singular value of [0, 1] could pass 16 before the last step or 256 after it (or one of
+    b A + c A^2 256) are refused.  X starts exact to 2^-40: a matrix of a norm far below eps, of which next to nothing is
+    left, loses a share of sqrt(m n) 2^-40 eps / |x|_F of it."""
     dtype = _element_type(x, "x")
     if x.dim() < 2:
         raise RuntimeError(f"orthogonalize: x {tuple(x.shape)} must have at least two dimensions")

@@ -1,6 +1,8 @@
 """Orthogonalised updates: calls that once went wrong (batches of more matrices than one launch's extent holds,
 bf16 results with products of fewer bits than asked for, small matrices whose arithmetic their neighbours decided,
 coefficients that shrink the iterates below what fp16 parts held, masked weights)."""
+import math
+
 import pytest
 import torch
 
@@ -121,3 +123,14 @@ def test_masked_weights_stay_zero(graph):
         off_mask = mask.to(DEV) == 0
         assert bool((got[k][off_mask] == 0).all()), k
         assert bool((got[k][~off_mask] != p0[~off_mask]).float().mean() > 0.9), k
+
+
+@pytest.mark.parametrize("shape", [(68, 68), (200, 300)], ids=str)
+@pytest.mark.parametrize("below", [1e-2, 1e-4, 1e-6])
+def test_norm_far_below_eps(shape, below):
+    """X_0 is exact to 2^-40 in each entry, and the iterates that grow from it to half of that again."""
+    x, eps = gaussian(*shape, seed=8), 1e-3
+    x = x * (below * eps / float(x.norm()))
+    got, want = ops.orthogonalize(x.to(DEV), eps=eps).double().cpu(), exact(x, eps=eps)
+    share = 2 * math.sqrt(x.numel()) * 2.0 ** -40 * eps / float(x.double().norm())
+    assert float((got - want).norm()) <= (TOL32 + share) * float(want.norm())
