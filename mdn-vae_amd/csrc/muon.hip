@@ -11,7 +11,8 @@
 // the directions of small singular values; B maps into the span of the large ones, so errors of A, of B and of the
 // product B X hardly reach those directions - only the rounding of X itself and of a X does.  The epilogue therefore
 // adds a X in fp32 from both parts.  Measured against float64 this is at or below the error of the same iteration in
-// plain fp32 (1e-6 .. 6e-6 of the norm, by spectrum).  One product of the high parts only (a X still from both) is the
+// plain fp32 (1e-6 .. 6e-6 of the norm, by spectrum; 1024 x 4624 of rank 16, whose empty directions hold nothing but
+// rounding, 3.3e-5 and 5.1e-5).  One product of the high parts only (a X still from both) is the
 // caller's choice: 0.3e-3 .. 1.9e-3 of the norm by itself, which takes a bf16 result of 1024 x 4624 Gaussian entries from 1.66e-3
 // (its own rounding, with all parts) to 2.14e-3.
 //
